@@ -20,7 +20,8 @@ OUT = os.path.join(HERE, "gpullama_attn", "libgpullama_attn.so")
 INCLUDE = os.path.normpath(os.path.join(HERE, "..", "include"))
 
 SOURCES = ["api.cu", "decode.cu", "combine.cu", "rope.cu", "prefill.cu", "comm.cpp", "peer.cpp",
-           "noalloc.cu", "ingest.cu", "wo.cu", "q8.cu", "debug.cu"]
+           "noalloc.cu", "ingest.cu", "wo.cu", "q8.cu", "debug.cu", "api_cache.cu",
+           "block_bounds.cu", "append_batched.cu", "block_select.cu", "row_attend.cu", "evict.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
               "-I", INCLUDE]

@@ -14,69 +14,12 @@
 
 #include "gpullama_attn.h"
 #include "gla_common.cuh"
-#include "gla_internal.h"
-#include "gla_comm.h"
-#include "gla_peer.h"
+#include "gla_ctx.h"
 #include "gla_xch.h"
 
-struct gla_ctx {
-  int device = 0;
-  cudaStream_t stream = nullptr;
-  gla::DeviceInfo dev{};
-  int32_t* status = nullptr;        // device status word
-  int32_t* counters = nullptr;      // piece counters (zero between calls)
-  size_t counters_cap = 0;
-  uint64_t* parts = nullptr;        // piece slots (tagged 64-bit words, zeroed at allocation)
-  size_t parts_cap = 0;             // words
-  uint64_t* trace = nullptr;        // GLA_OPT_TRACE: per-CTA phase stamps of the last decode
-  size_t trace_words = 0;
-  float* records = nullptr;         // sharded decode: local records
-  float* gathered = nullptr;        // sharded decode: all ranks' records
-  size_t records_cap = 0;           // floats per rank
-  uint16_t* ingest_ws = nullptr;    // prompt ingestion: FP16 q (and K/V) copies
-  size_t ingest_cap = 0;            // halves
-  gla::Comm comm;
-  gla::PeerExchange xch;            // sharded decode: peer exchange buffers
-  int32_t opt_early_kv = 2;         // GLA_OPT_EARLY_KV_PREFETCH
-  int32_t opt_shard_exchange = 1;   // GLA_OPT_SHARD_EXCHANGE
-  std::string last_error;
-};
+using namespace gla;  // fail, cuda_fail, aligned16, DeviceGuard, stream_capturing
 
 namespace {
-
-int fail(gla_ctx* ctx, int code, const std::string& msg) {
-  if (ctx) ctx->last_error = msg;
-  return code;
-}
-
-int cuda_fail(gla_ctx* ctx, cudaError_t e, const char* what) {
-  return fail(ctx, GLA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// The context's 256-byte status block: the device status word at 0, the
-// decode call-epoch word (see DecodeWorkspace) at kEpochOffset.
-constexpr size_t kEpochOffset = 64;
-
-// Makes the context's device current for the duration of a call.
-struct DeviceGuard {
-  int prev = -1;
-  bool ok = true;
-  explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-    if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
-  }
-  ~DeviceGuard() {
-    if (prev >= 0) cudaSetDevice(prev);
-  }
-};
-
-bool stream_capturing(cudaStream_t s) {
-  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(s, &st) != cudaSuccess) return false;
-  return st != cudaStreamCaptureStatusNone;
-}
 
 // Grows the piece workspace; never during stream capture.
 int ensure_workspace(gla_ctx* ctx, size_t part_words, size_t counters) {
@@ -452,6 +395,8 @@ int32_t gla_destroy(gla_ctx* ctx) {
     cudaFree(ctx->gathered);
     cudaFree(ctx->ingest_ws);
     cudaFree(ctx->trace);
+    cudaFree(ctx->scores);
+    for (void* p : ctx->retired) cudaFree(p);
   }
   delete ctx;
   return rc;

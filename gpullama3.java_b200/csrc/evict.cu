@@ -1,0 +1,281 @@
+// evict.cu - eviction from a KV cache by accumulated attention weight.
+//
+// Of a sequence's n rows each kv head keeps n_keep: the n_recent newest, and
+// of the older ones those with the largest accumulated weight
+// (gla_decode_weights_*), ties to the oldest.  Kept rows stay in order and
+// move to rows 0..n_keep-1, each kv head by itself (its columns of a cache
+// row), and their weights with them.  Rows carry their RoPE'd keys, so
+// attention over the kept rows needs no positions.
+//
+// Which rows: a cluster of CTAs a (sequence, kv head) selects over the weights
+// with the radix selection of cache_ops.cuh and writes the ascending list.
+// The rows then move in a second kernel (HBM-bound, each kept row read and
+// written once): to another cache, every (row, 16-byte chunk) by itself; in
+// place, in rounds (below).
+#include "cache_ops.cuh"
+
+namespace gla {
+
+namespace {
+
+constexpr int kSelThreads = 512;
+constexpr int kMoveThreads = 256;
+
+__global__ void __launch_bounds__(kSelThreads)
+    evict_select_kernel(const float* const* __restrict__ weight_ptrs, int64_t weight_stride,
+                        const int32_t* __restrict__ n_pos, int32_t max_n_pos, int32_t n_keep,
+                        int32_t n_recent, int32_t* __restrict__ kept, int32_t n_kv, int S,
+                        int32_t* __restrict__ status) {
+  __shared__ SelectScratch sh;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int tid = threadIdx.x;
+  const int rank = S > 1 ? (int)(blockIdx.x % (unsigned)S) : 0;
+  const int item = (int)(blockIdx.x / (unsigned)S);
+  const int b = item / n_kv, g = item - b * n_kv;
+  int32_t n = clamped_rows(n_pos, b, max_n_pos, status);
+  const float* w = weight_ptrs[b];
+  if (!usable_weights(w, status)) n = 0;
+  int32_t* out = kept + (int64_t)item * n_keep;
+  if (n <= n_keep) {  // nothing to evict
+    for (int32_t i = rank * kSelThreads + tid; i < n_keep; i += S * kSelThreads)
+      out[i] = i < n ? i : -1;
+    return;  // every CTA of the cluster takes this way
+  }
+  const int32_t older = n - n_recent, pick = n_keep - n_recent;
+  for (int32_t i = rank * kSelThreads + tid; i < n_recent; i += S * kSelThreads)
+    out[pick + i] = older + i;
+  if (pick == 0) return;
+  int32_t lo, hi;
+  share_of(older, S, rank, &lo, &hi);
+  const float* mine = w + (int64_t)g * weight_stride + lo;
+  cluster_select<kSelThreads, uint32_t>(
+      sh, S, rank, hi - lo, (uint32_t)pick, [&](int32_t i) { return order_key(mine[i]); },
+      [&](int32_t i, uint32_t at) { out[at] = lo + i; });
+}
+
+// Kept rows of one kv head to another cache: thread = (row, 16-byte chunk).
+template <int kChunks, int kPer, class T>
+__global__ void __launch_bounds__(kMoveThreads)
+    evict_copy_kernel(T* const* __restrict__ k_ptrs, T* const* __restrict__ v_ptrs,
+                      float* const* __restrict__ weight_ptrs, int64_t weight_stride,
+                      T* const* __restrict__ k_out_ptrs, T* const* __restrict__ v_out_ptrs,
+                      float* const* __restrict__ weight_out_ptrs, int64_t weight_out_stride,
+                      const int32_t* __restrict__ n_pos, int32_t max_n_pos, int32_t n_keep,
+                      const int32_t* __restrict__ kept, int32_t n_kv, int64_t kv_stride,
+                      int32_t parts, int32_t* __restrict__ status) {
+  constexpr int kUnroll = 4;
+  constexpr int kRows = kMoveThreads * kUnroll / kChunks;  // rows of a CTA
+  pdl_wait();
+  const int tid = threadIdx.x;
+  const int item = (int)(blockIdx.x / (unsigned)parts), part = (int)(blockIdx.x % (unsigned)parts);
+  const int b = item / n_kv, g = item - b * n_kv;
+  const int32_t n = clamped_rows(n_pos, b, max_n_pos, status);
+  const T* k = k_ptrs[b];
+  const T* v = v_ptrs[b];
+  const float* w = weight_ptrs[b];
+  T* ko = k_out_ptrs[b];
+  T* vo = v_out_ptrs[b];
+  float* wo = weight_out_ptrs[b];
+  if (!usable_ptrs(k, v, status) || !usable_ptrs(ko, vo, status) || !usable_weights(w, status) ||
+      !usable_weights(wo, status))
+    return;
+  if (k == ko || v == vo || w == wo) {  // another order of moves is needed in place
+    if (tid == 0) atomicCAS(status, 0, GLA_ERR_INVALID_ARG);
+    return;
+  }
+  const int32_t m = min(n, n_keep);
+  const int32_t row0 = part * kRows;
+  if (row0 >= m) return;
+  const int32_t* list = kept + (int64_t)item * n_keep;
+  float4 xk[kUnroll], xv[kUnroll];
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int i = u * kMoveThreads + tid;
+    const int r = i / kChunks, c = i - r * kChunks;
+    if (r < kRows && row0 + r < m) {
+      const int64_t src =
+          (int64_t)list[row0 + r] * kv_stride + (int64_t)g * kChunks * kPer + c * kPer;
+      xk[u] = __ldcg(reinterpret_cast<const float4*>(k + src));
+      xv[u] = __ldcg(reinterpret_cast<const float4*>(v + src));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const int i = u * kMoveThreads + tid;
+    const int r = i / kChunks, c = i - r * kChunks;
+    if (r < kRows && row0 + r < m) {
+      const int64_t dst = (int64_t)(row0 + r) * kv_stride + (int64_t)g * kChunks * kPer + c * kPer;
+      *reinterpret_cast<float4*>(ko + dst) = xk[u];
+      *reinterpret_cast<float4*>(vo + dst) = xv[u];
+    }
+  }
+  for (int r = tid; r < kRows && row0 + r < m; r += kMoveThreads)
+    wo[(int64_t)g * weight_out_stride + row0 + r] = w[(int64_t)g * weight_stride + list[row0 + r]];
+}
+
+// In place.  One CTA moves a column slice of 64 bytes (4 chunks) of K or of V
+// of one (sequence, kv head), or its weights, so slices never touch each
+// other's bytes.  Rows move in rounds of kRound list entries: all loads of a
+// round, a barrier, its stores.  A kept row's source is never below its
+// destination (list[i] >= i, ascending), so the stores of round r, to rows
+// below (r + 1) kRound, can only hit sources of rounds <= r, which are all
+// loaded; the loads of round r + 1 may therefore be in flight meanwhile.
+template <int kSlices, int kPer, class T>
+__global__ void __launch_bounds__(kMoveThreads)
+    evict_compact_kernel(T* const* __restrict__ k_ptrs, T* const* __restrict__ v_ptrs,
+                         float* const* __restrict__ weight_ptrs, int64_t weight_stride,
+                         const int32_t* __restrict__ n_pos, int32_t max_n_pos, int32_t n_keep,
+                         const int32_t* __restrict__ kept, int32_t n_kv, int64_t kv_stride,
+                         int32_t* __restrict__ status) {
+  constexpr int kUnroll = 8;
+  constexpr int kStep = kMoveThreads / 4;       // rows side by side
+  constexpr int kRound = kStep * kUnroll;
+  constexpr int kParts = 2 * kSlices + 1;       // K slices, V slices, weights
+  pdl_wait();
+  const int tid = threadIdx.x;
+  const int item = (int)(blockIdx.x / kParts), part = (int)(blockIdx.x % kParts);
+  const int b = item / n_kv, g = item - b * n_kv;
+  const int32_t n = clamped_rows(n_pos, b, max_n_pos, status);
+  if (n <= n_keep) return;
+  T* k = k_ptrs[b];
+  T* v = v_ptrs[b];
+  float* w = weight_ptrs[b];
+  if (!usable_ptrs(k, v, status) || !usable_weights(w, status)) return;
+  const int32_t* list = kept + (int64_t)item * n_keep;
+  if (part == kParts - 1) {
+    w += (int64_t)g * weight_stride;
+    constexpr int kWr = kMoveThreads * kUnroll;
+    for (int32_t i0 = 0; i0 < n_keep; i0 += kWr) {
+      float x[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int32_t i = i0 + u * kMoveThreads + tid;
+        if (i < n_keep) x[u] = __ldcg(w + list[i]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int32_t i = i0 + u * kMoveThreads + tid;
+        if (i < n_keep) w[i] = x[u];
+      }
+    }
+    // the rows behind have no weight yet: a token appended there starts at zero
+    __syncthreads();
+    for (int32_t i = n_keep + tid; i < n; i += kMoveThreads) w[i] = 0.f;
+    return;
+  }
+  T* base = (part < kSlices ? k : v) + (int64_t)g * kSlices * 4 * kPer +
+            (part % kSlices) * 4 * kPer + (tid & 3) * kPer;
+  const int r0 = tid >> 2;
+  float4 cur[kUnroll], nxt[kUnroll];
+  int32_t from[kUnroll], from_next[kUnroll];
+  auto load = [&](int32_t i0, float4 (&x)[kUnroll], int32_t (&src)[kUnroll]) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int32_t i = i0 + u * kStep + r0;
+      src[u] = i < n_keep ? list[i] : i;
+      // a row that stays needs no move
+      if (src[u] != i) x[u] = __ldcg(reinterpret_cast<const float4*>(base + (int64_t)src[u] * kv_stride));
+    }
+  };
+  load(0, cur, from);
+  for (int32_t i0 = 0; i0 < n_keep; i0 += kRound) {
+    __syncthreads();  // every load of this round is done
+    if (i0 + kRound < n_keep) load(i0 + kRound, nxt, from_next);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int32_t i = i0 + u * kStep + r0;
+      if (from[u] != i) *reinterpret_cast<float4*>(base + (int64_t)i * kv_stride) = cur[u];
+      cur[u] = nxt[u];
+      from[u] = from_next[u];
+    }
+  }
+}
+
+template <class... Params, class... Args>
+int launch_pdl(void (*kern)(Params...), unsigned grid, int threads, cudaStream_t stream,
+               const char* what, std::string* err, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    *err = std::string(what) + " launch failed: " + cudaGetErrorString(e);
+    return GLA_ERR_CUDA;
+  }
+  return GLA_OK;
+}
+
+template <class T, int HD>
+int launch_move(const EvictRequest& r, cudaStream_t stream, std::string* err) {
+  constexpr int kPer = 16 / sizeof(T);
+  constexpr int kChunks = HD / kPer;
+  const int64_t items = (int64_t)r.batch * r.n_kv;
+  if (r.k_out_ptrs) {
+    constexpr int kRows = kMoveThreads * 4 / kChunks;
+    const int32_t most = std::min(r.n_keep, r.max_n_pos);
+    const int64_t parts = std::max(1, (most + kRows - 1) / kRows);
+    if (items * parts > INT32_MAX) {
+      *err = "too many rows to move in one call";
+      return GLA_ERR_NOT_SUPPORTED;
+    }
+    return launch_pdl(evict_copy_kernel<kChunks, kPer, T>, (unsigned)(items * parts), kMoveThreads,
+                      stream, "evict copy", err, reinterpret_cast<T* const*>(r.k_ptrs),
+                      reinterpret_cast<T* const*>(r.v_ptrs), r.weight_ptrs, r.weight_stride,
+                      reinterpret_cast<T* const*>(r.k_out_ptrs),
+                      reinterpret_cast<T* const*>(r.v_out_ptrs), r.weight_out_ptrs,
+                      r.weight_out_stride, r.n_pos, r.max_n_pos, r.n_keep,
+                      (const int32_t*)r.kept, r.n_kv, r.kv_stride, (int32_t)parts, r.status);
+  }
+  constexpr int kSlices = kChunks / 4;
+  const int64_t grid = items * (2 * kSlices + 1);
+  if (grid > INT32_MAX) {
+    *err = "batch * n_kv_heads too large";
+    return GLA_ERR_NOT_SUPPORTED;
+  }
+  return launch_pdl(evict_compact_kernel<kSlices, kPer, T>, (unsigned)grid, kMoveThreads, stream,
+                    "evict compaction", err, reinterpret_cast<T* const*>(r.k_ptrs),
+                    reinterpret_cast<T* const*>(r.v_ptrs), r.weight_ptrs, r.weight_stride, r.n_pos,
+                    r.max_n_pos, r.n_keep, (const int32_t*)r.kept, r.n_kv, r.kv_stride, r.status);
+}
+
+template <class T>
+int move_dim(const EvictRequest& r, cudaStream_t stream, std::string* err) {
+  switch (r.head_dim) {
+    case 64: return launch_move<T, 64>(r, stream, err);
+    case 96: return launch_move<T, 96>(r, stream, err);
+    default: return launch_move<T, 128>(r, stream, err);
+  }
+}
+
+}  // namespace
+
+int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stream,
+                 std::string* err) {
+  static std::atomic<uint64_t> attr_done{0};
+  const int64_t items = (int64_t)r.batch * r.n_kv;
+  // a CTA for every 2048 weights, as long as that does not exceed the device
+  int S = 1;
+  while (S < 16 && items * S < dev.sms && r.max_n_pos > (int64_t)2048 * S) S *= 2;
+  if (items * S > INT32_MAX) {
+    *err = "batch * n_kv_heads too large";
+    return GLA_ERR_NOT_SUPPORTED;
+  }
+  int rc = launch_clusters(evict_select_kernel, (unsigned)(items * S), kSelThreads, 0, S, attr_done,
+                           stream, "evict selection", err,
+                           (const float* const*)r.weight_ptrs, r.weight_stride, r.n_pos,
+                           r.max_n_pos, r.n_keep, r.n_recent, r.kept, r.n_kv, S, r.status);
+  if (rc != GLA_OK) return rc;
+  return r.dtype == GLA_DTYPE_F16 ? move_dim<__half>(r, stream, err)
+                                  : move_dim<float>(r, stream, err);
+}
+
+}  // namespace gla

@@ -129,6 +129,102 @@ int launch_ingest(bool f16_cache, const float* q, const float* k, const float* v
                   int32_t rope_style, int32_t* status, const DeviceInfo& dev,
                   cudaStream_t stream, std::string* err);
 
+// Long caches: bounds of key blocks, batched append, block selection,
+// attention over listed blocks or over all rows with its weights added up,
+// and eviction.  dtype: GLA_DTYPE_F32 or GLA_DTYPE_F16 (the caches');
+// pointer arrays are device arrays of `batch` device pointers.
+struct BoundsRequest {  // block_bounds.cu
+  int dtype;
+  const void* const* k_ptrs;
+  const int32_t* start_pos;    // null: all blocks
+  const int32_t* n_pos;
+  int32_t max_n_pos;
+  void* const* bounds_ptrs;
+  int32_t batch, n_kv, head_dim;
+  int64_t kv_stride;
+  int32_t block_rows;          // 16, 32, 64 or 128
+  int32_t* status;
+};
+int launch_block_bounds(const BoundsRequest& r, cudaStream_t stream, std::string* err);
+
+struct AppendRequest {  // append_batched.cu
+  int dtype;
+  const float* q;
+  const float* k;
+  const float* v;
+  float* q_out;
+  void* const* k_ptrs;
+  void* const* v_ptrs;
+  const int32_t* positions;
+  const int32_t* rows;         // null: positions
+  void* const* bounds_ptrs;    // null: none
+  int32_t block_rows;          // with bounds_ptrs
+  int32_t batch, n_heads, n_kv, head_dim;
+  int64_t kv_stride;
+  int32_t context_length;
+  double theta;
+  int32_t rope_style;
+  int32_t* status;
+};
+int launch_append_batched(const AppendRequest& r, cudaStream_t stream, std::string* err);
+
+struct SelectRequest {  // block_select.cu
+  int dtype;
+  const float* q;
+  const void* const* bounds_ptrs;
+  const int32_t* n_pos;
+  int32_t max_n_pos;
+  int32_t* block_ids;
+  int32_t batch, n_heads, n_kv, head_dim;
+  int32_t block_rows, n_sel, n_first, n_last;
+  int32_t* status;
+};
+int launch_block_select(const SelectRequest& r, const DeviceInfo& dev, cudaStream_t stream,
+                        std::string* err);
+
+struct AttendRequest {  // row_attend.cu
+  int dtype;
+  const float* q;
+  const void* const* k_ptrs;
+  const void* const* v_ptrs;
+  const int32_t* n_pos;
+  int32_t max_n_pos;
+  float* xb;
+  int32_t batch, n_heads, n_kv, head_dim;
+  int64_t kv_stride;
+  float scale;
+  const int32_t* block_ids = nullptr;  // listed blocks: [batch][n_kv][n_sel]
+  int32_t n_sel = 0;
+  int32_t block_rows = 0;
+  float* const* weight_ptrs = nullptr;  // all rows, weights added: [n_kv][weight_stride] each
+  int64_t weight_stride = 0;
+  float* scores = nullptr;              // workspace of attend_score_floats(...) floats
+  int32_t* status;
+};
+size_t attend_score_floats(const AttendRequest& r);
+int launch_attend(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,
+                  std::string* err);
+
+struct EvictRequest {  // evict.cu
+  int dtype;
+  void* const* k_ptrs;
+  void* const* v_ptrs;
+  float* const* weight_ptrs;
+  int64_t weight_stride;
+  const int32_t* n_pos;
+  int32_t max_n_pos, n_keep, n_recent;
+  int32_t* kept;                        // [batch][n_kv][n_keep]
+  void* const* k_out_ptrs;              // null (all three): in place
+  void* const* v_out_ptrs;
+  float* const* weight_out_ptrs;
+  int64_t weight_out_stride;
+  int32_t batch, n_kv, head_dim;
+  int64_t kv_stride;
+  int32_t* status;
+};
+int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stream,
+                 std::string* err);
+
 // Test hook (debug.cu): a PDL kernel that releases its dependents at once,
 // spins delay_us (at most 1000) and then adds delta to *position_holder.
 int launch_advance_position(int32_t* position_holder, int32_t delta, int32_t delay_us,

@@ -99,6 +99,17 @@ _SIGS = {
     "gla_ingest_prompt_f16kv": (_I32, [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I32,
                                        _I32, _F, _I32]),
 }
+for _t in ("f32kv", "f16kv"):  # long caches
+    _SIGS.update({
+        f"gla_block_bounds_{_t}": (_I32, [_P, _P, _P, _P, _I32, _P, _I32, _I32, _I32, _I64, _I32]),
+        f"gla_rope_append_batched_{_t}": (_I32, [_P] * 10 + [_I32] * 5 + [_I64, _I32, _F, _I32]),
+        f"gla_block_select_{_t}": (_I32, [_P, _P, _P, _P, _I32, _P] + [_I32] * 8),
+        f"gla_decode_blocks_{_t}": (_I32, [_P] * 6 + [_I32, _P] + [_I32] * 4 + [_I64, _I32, _F]),
+        f"gla_decode_weights_{_t}": (_I32, [_P] * 5 + [_I32, _P, _P, _I64] + [_I32] * 4
+                                     + [_I64, _F]),
+        f"gla_kv_evict_{_t}": (_I32, [_P] * 4 + [_I64, _P] + [_I32] * 3 + [_P] * 4 + [_I64]
+                               + [_I32] * 3 + [_I64]),
+    })
 
 EXPORTED_SYMBOLS = tuple(_SIGS)
 
@@ -433,3 +444,76 @@ class Context:
                                                 _ptr(key_cache), _ptr(value_cache), n_heads,
                                                 n_kv_heads, head_dim, _ptr(position_holder),
                                                 theta, style), "gla_rope_append_f32")
+
+    # -- long caches ------------------------------------------------------------
+    def block_bounds(self, k_ptrs, n_pos, max_n_pos, bounds_ptrs, batch, n_kv_heads, head_dim,
+                     block_rows, start_pos=None, kv_stride=None, f16_cache=False):
+        """gla_block_bounds_*: smallest and largest key of every block and channel."""
+        if kv_stride is None:
+            kv_stride = n_kv_heads * head_dim
+        fn = self._L.gla_block_bounds_f16kv if f16_cache else self._L.gla_block_bounds_f32kv
+        self._check(fn(self._h, _ptr(k_ptrs), _ptr(start_pos), _ptr(n_pos), max_n_pos,
+                       _ptr(bounds_ptrs), batch, n_kv_heads, head_dim, kv_stride, block_rows),
+                    "gla_block_bounds")
+
+    def rope_append_batched(self, q, k, v, q_out, k_ptrs, v_ptrs, positions, batch, n_heads,
+                            n_kv_heads, head_dim, context_length, theta, style=ROPE_INTERLEAVED,
+                            rows=None, bounds_ptrs=None, block_rows=0, kv_stride=None,
+                            f16_cache=False):
+        """gla_rope_append_batched_*: the new token of every sequence into its cache row."""
+        if kv_stride is None:
+            kv_stride = n_kv_heads * head_dim
+        fn = (self._L.gla_rope_append_batched_f16kv if f16_cache
+              else self._L.gla_rope_append_batched_f32kv)
+        self._check(fn(self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_ptrs),
+                       _ptr(v_ptrs), _ptr(positions), _ptr(rows), _ptr(bounds_ptrs), block_rows,
+                       batch, n_heads, n_kv_heads, head_dim, kv_stride, context_length, theta,
+                       style), "gla_rope_append_batched")
+
+    def block_select(self, q, bounds_ptrs, n_pos, max_n_pos, block_ids, batch, n_heads,
+                     n_kv_heads, head_dim, block_rows, n_sel, n_first=0, n_last=1,
+                     f16_cache=False):
+        """gla_block_select_*: ids of the blocks each query's kv heads read."""
+        fn = self._L.gla_block_select_f16kv if f16_cache else self._L.gla_block_select_f32kv
+        self._check(fn(self._h, _ptr(q), _ptr(bounds_ptrs), _ptr(n_pos), max_n_pos,
+                       _ptr(block_ids), batch, n_heads, n_kv_heads, head_dim, block_rows, n_sel,
+                       n_first, n_last), "gla_block_select")
+
+    def decode_blocks(self, q, k_ptrs, v_ptrs, n_pos, block_ids, n_sel, xb, batch, n_heads,
+                      n_kv_heads, head_dim, block_rows, scale=None, kv_stride=None,
+                      f16_cache=False):
+        """gla_decode_blocks_*: attention over the listed blocks of rows."""
+        if scale is None:
+            scale = 1.0 / math.sqrt(head_dim)
+        if kv_stride is None:
+            kv_stride = n_kv_heads * head_dim
+        fn = self._L.gla_decode_blocks_f16kv if f16_cache else self._L.gla_decode_blocks_f32kv
+        self._check(fn(self._h, _ptr(q), _ptr(k_ptrs), _ptr(v_ptrs), _ptr(n_pos),
+                       _ptr(block_ids), n_sel, _ptr(xb), batch, n_heads, n_kv_heads, head_dim,
+                       kv_stride, block_rows, scale), "gla_decode_blocks")
+
+    def decode_weights(self, q, k_ptrs, v_ptrs, n_pos, max_n_pos, xb, weight_ptrs, weight_stride,
+                       batch, n_heads, n_kv_heads, head_dim, scale=None, kv_stride=None,
+                       f16_cache=False):
+        """gla_decode_weights_*: attention over all rows, each row's weight added up."""
+        if scale is None:
+            scale = 1.0 / math.sqrt(head_dim)
+        if kv_stride is None:
+            kv_stride = n_kv_heads * head_dim
+        fn = self._L.gla_decode_weights_f16kv if f16_cache else self._L.gla_decode_weights_f32kv
+        self._check(fn(self._h, _ptr(q), _ptr(k_ptrs), _ptr(v_ptrs), _ptr(n_pos), max_n_pos,
+                       _ptr(xb), _ptr(weight_ptrs), weight_stride, batch, n_heads, n_kv_heads,
+                       head_dim, kv_stride, scale), "gla_decode_weights")
+
+    def kv_evict(self, k_ptrs, v_ptrs, weight_ptrs, weight_stride, n_pos, max_n_pos, n_keep,
+                 n_recent, kept, batch, n_kv_heads, head_dim, k_out_ptrs=None, v_out_ptrs=None,
+                 weight_out_ptrs=None, weight_out_stride=0, kv_stride=None, f16_cache=False):
+        """gla_kv_evict_*: keeps the newest rows and those of the largest weight, in place
+        or in other caches."""
+        if kv_stride is None:
+            kv_stride = n_kv_heads * head_dim
+        fn = self._L.gla_kv_evict_f16kv if f16_cache else self._L.gla_kv_evict_f32kv
+        self._check(fn(self._h, _ptr(k_ptrs), _ptr(v_ptrs), _ptr(weight_ptrs), weight_stride,
+                       _ptr(n_pos), max_n_pos, n_keep, n_recent, _ptr(kept), _ptr(k_out_ptrs),
+                       _ptr(v_out_ptrs), _ptr(weight_out_ptrs), weight_out_stride, batch,
+                       n_kv_heads, head_dim, kv_stride), "gla_kv_evict")

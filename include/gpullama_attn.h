@@ -476,6 +476,165 @@ int32_t gla_rope_append_f32(gla_ctx* ctx, float* q, float* k, const float* v, fl
                             int32_t rope_style);
 
 /* ------------------------------------------------------------------------ */
+/* Long caches: read in part, kept in part                                   */
+/* ------------------------------------------------------------------------ */
+
+/* Batched operators for sequences whose caches are too long to read, or to
+ * keep, whole.  No reference counterparts (the reference reads every cached
+ * position: InferenceCore.java:105-144).
+ *   gla_block_bounds_*        bounds of the keys of every block of rows
+ *   gla_rope_append_batched_* the new token of every sequence into its cache
+ *   gla_block_select_*        the blocks each query's kv heads read
+ *   gla_decode_blocks_*       attention over those blocks
+ *   gla_decode_weights_*      attention over all rows, its weights added up
+ *   gla_kv_evict_*            the rows of the largest weights kept, the rest dropped
+ * Common to all of them:
+ *  - *_ptrs are DEVICE arrays of `batch` device pointers, one a sequence, 16-byte
+ *    aligned (weights: 4-byte); _f32kv / _f16kv is the type of the caches and of
+ *    their bounds.  A null or misaligned pointer latches GLA_ERR_INVALID_ARG /
+ *    GLA_ERR_ALIGNMENT in the device status and that sequence is skipped (an
+ *    attention output is then zero).
+ *  - k/v caches: row t of kv head g at t*kv_stride + g*head_dim, as
+ *    gla_decode_batched_*; kv_stride a multiple of 16 bytes; head_dim 64, 96 or
+ *    128; kvMul = n_heads / n_kv_heads at most 8; any batch.
+ *  - n_pos: DEVICE int32 [batch], the rows a sequence has, 0 to max_n_pos (host).
+ *    A value outside is clamped and latches GLA_ERR_INVALID_ARG in the device
+ *    status.  Rows at and past n_pos are never read nor written, so what they
+ *    hold (an infinity, a NaN) does not matter.
+ *  - block_rows (16, 32, 64 or 128): block j is rows [j*block_rows, (j+1)*block_rows).
+ *  - Results do not depend on timing: two calls on the same input give the
+ *    same bits.
+ *  - Calls can be captured in a CUDA graph; gla_decode_weights_* uses a context
+ *    workspace that must have grown before (run its largest call once), so
+ *    graphs of one context that hold it must not run at the same time. */
+
+/* bounds: [n_blocks][n_kv_heads][2][head_dim] a sequence: the smallest (0) and the
+ * largest (1) key of each channel over the rows t < n_pos of a block.  Exact; a NaN
+ * key is ignored unless all keys of its channel are NaN.  start_pos (DEVICE int32
+ * [batch], or NULL for 0): rows before it are unchanged, so only blocks from
+ * start_pos / block_rows on are written.  Blocks past the last row are left as they
+ * were. */
+int32_t gla_block_bounds_f32kv(gla_ctx* ctx, const float* const* k_ptrs, const int32_t* start_pos,
+                               const int32_t* n_pos, int32_t max_n_pos, float* const* bounds_ptrs,
+                               int32_t batch, int32_t n_kv_heads, int32_t head_dim,
+                               int64_t kv_stride, int32_t block_rows);
+int32_t gla_block_bounds_f16kv(gla_ctx* ctx, const uint16_t* const* k_ptrs,
+                               const int32_t* start_pos, const int32_t* n_pos, int32_t max_n_pos,
+                               uint16_t* const* bounds_ptrs, int32_t batch, int32_t n_kv_heads,
+                               int32_t head_dim, int64_t kv_stride, int32_t block_rows);
+
+/* The new token of every sequence: q [batch][n_heads*head_dim] rotated into q_out
+ * (may be q), k [batch][kv_dim] rotated for positions[b] (DEVICE int32) and written
+ * with v to cache row rows[b] (DEVICE int32; NULL: the position).  Row and position
+ * differ once rows were evicted.  RoPE and its roundings as gla_rope_append_f32; an
+ * FP16 cache gets k and v rounded to nearest.  bounds_ptrs (or NULL): the bounds of
+ * the row's block are brought up to date - set to the new key if it is the block's
+ * first row, else widened by it - so appending row after row keeps them equal to
+ * gla_block_bounds_* (a row written again leaves them as wide as before).  Batch
+ * entries may share a cache if their rows differ and, with bounds, their blocks.
+ * Rows outside [0, context_length) or negative positions: nothing of that sequence
+ * is written and GLA_ERR_INVALID_ARG is latched in the device status. */
+int32_t gla_rope_append_batched_f32kv(gla_ctx* ctx, const float* q, const float* k, const float* v,
+                                      float* q_out, float* const* k_ptrs, float* const* v_ptrs,
+                                      const int32_t* positions, const int32_t* rows,
+                                      float* const* bounds_ptrs, int32_t block_rows, int32_t batch,
+                                      int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                      int64_t kv_stride, int32_t context_length, float theta,
+                                      int32_t rope_style);
+int32_t gla_rope_append_batched_f16kv(gla_ctx* ctx, const float* q, const float* k, const float* v,
+                                      float* q_out, uint16_t* const* k_ptrs,
+                                      uint16_t* const* v_ptrs, const int32_t* positions,
+                                      const int32_t* rows, uint16_t* const* bounds_ptrs,
+                                      int32_t block_rows, int32_t batch, int32_t n_heads,
+                                      int32_t n_kv_heads, int32_t head_dim, int64_t kv_stride,
+                                      int32_t context_length, float theta, int32_t rope_style);
+
+/* The n_sel blocks that each (query, kv head) reads: block_ids [batch][n_kv_heads]
+ * [n_sel] (DEVICE int32), ascending, -1 behind the last one.  Of the n_blocks =
+ * ceil(n_pos / block_rows) blocks the first n_first and the last n_last are always
+ * chosen (n_first + n_last <= n_sel), the others by
+ *     score(j, g) = max over the q heads h of g of
+ *                   sum_d (min(q_hd, 0) lo_jgd + max(q_hd, 0) hi_jgd),
+ * an upper bound of q_h . k_t over block j's rows (for a positive scale), summed in
+ * FP64; the highest are chosen, ties to the lowest block, a head whose sum is NaN (an
+ * infinite bound times zero is) counts as the lowest.  With n_blocks <= n_sel all are
+ * chosen.  Batch entries may share bounds: the queries of
+ * a prompt chunk over one cache, each with its own n_pos and blocks. */
+int32_t gla_block_select_f32kv(gla_ctx* ctx, const float* q, const float* const* bounds_ptrs,
+                               const int32_t* n_pos, int32_t max_n_pos, int32_t* block_ids,
+                               int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                               int32_t head_dim, int32_t block_rows, int32_t n_sel,
+                               int32_t n_first, int32_t n_last);
+int32_t gla_block_select_f16kv(gla_ctx* ctx, const float* q, const uint16_t* const* bounds_ptrs,
+                               const int32_t* n_pos, int32_t max_n_pos, int32_t* block_ids,
+                               int32_t batch, int32_t n_heads, int32_t n_kv_heads,
+                               int32_t head_dim, int32_t block_rows, int32_t n_sel,
+                               int32_t n_first, int32_t n_last);
+
+/* Decode attention over listed blocks: as gla_decode_batched_*, but kv head g of
+ * batch entry b attends only to the rows below n_pos[b] of the blocks block_ids[b][g][0
+ * .. n_sel).  Negative ids and ids of blocks past the last row name no rows; a block
+ * listed twice counts twice; no row at all gives zeros.  n_sel * block_rows < 2^31.
+ * Batch entries may share caches (the queries of a prompt chunk). */
+int32_t gla_decode_blocks_f32kv(gla_ctx* ctx, const float* q, const float* const* k_ptrs,
+                                const float* const* v_ptrs, const int32_t* n_pos,
+                                const int32_t* block_ids, int32_t n_sel, float* xb, int32_t batch,
+                                int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                int64_t kv_stride, int32_t block_rows, float scale);
+int32_t gla_decode_blocks_f16kv(gla_ctx* ctx, const float* q, const uint16_t* const* k_ptrs,
+                                const uint16_t* const* v_ptrs, const int32_t* n_pos,
+                                const int32_t* block_ids, int32_t n_sel, float* xb, int32_t batch,
+                                int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                                int64_t kv_stride, int32_t block_rows, float scale);
+
+/* Decode attention over all rows, as gla_decode_batched_* (a sequence may have no
+ * rows: zeros), that also adds the weight each row got to a running sum:
+ *     w[g][t] += sum over the q heads h of kv head g of softmax_t(scale q_h . k_t),
+ * w = weight_ptrs[b], FP32 [n_kv_heads][weight_stride], weight_stride >= max_n_pos.
+ * Entries at and past n_pos are left as they were; set a row's entry to 0 when the
+ * row is appended.  Batch entries must not share weights.  Uses a context workspace
+ * of batch * n_heads * max_n_pos floats, grown on first use (not during stream
+ * capture). */
+int32_t gla_decode_weights_f32kv(gla_ctx* ctx, const float* q, const float* const* k_ptrs,
+                                 const float* const* v_ptrs, const int32_t* n_pos,
+                                 int32_t max_n_pos, float* xb, float* const* weight_ptrs,
+                                 int64_t weight_stride, int32_t batch, int32_t n_heads,
+                                 int32_t n_kv_heads, int32_t head_dim, int64_t kv_stride,
+                                 float scale);
+int32_t gla_decode_weights_f16kv(gla_ctx* ctx, const float* q, const uint16_t* const* k_ptrs,
+                                 const uint16_t* const* v_ptrs, const int32_t* n_pos,
+                                 int32_t max_n_pos, float* xb, float* const* weight_ptrs,
+                                 int64_t weight_stride, int32_t batch, int32_t n_heads,
+                                 int32_t n_kv_heads, int32_t head_dim, int64_t kv_stride,
+                                 float scale);
+
+/* Eviction: of a sequence's n_pos rows each kv head keeps n_keep - the n_recent newest
+ * (highest rows), and of the older ones those of the largest weight (weight_ptrs as
+ * for gla_decode_weights_*), ties to the lower row, a NaN lowest.  Kept rows keep their
+ * order and become rows 0..n_keep-1 of that kv head; their weights move with them.
+ * kept (DEVICE int32 [batch][n_kv_heads][n_keep]) receives the rows they were, -1 behind
+ * the last.  A sequence with n_pos <= n_keep keeps all.  The caller goes on with
+ * min(n_pos, n_keep) rows (and rebuilds the block bounds, if it uses them).
+ *  - k_out_ptrs, v_out_ptrs and weight_out_ptrs all NULL: in place; weights of the
+ *    rows [n_keep, n_pos) become 0, cache rows there are left as they were.
+ *  - all given: the kept rows and weights go there (caches of the same kv_stride,
+ *    weights [n_kv_heads][weight_out_stride], at least min(n_keep, max_n_pos)), the
+ *    sources stay.  The outputs must not overlap the sources; equal pointers latch
+ *    GLA_ERR_INVALID_ARG in the device status and that sequence is not moved. */
+int32_t gla_kv_evict_f32kv(gla_ctx* ctx, float* const* k_ptrs, float* const* v_ptrs,
+                           float* const* weight_ptrs, int64_t weight_stride, const int32_t* n_pos,
+                           int32_t max_n_pos, int32_t n_keep, int32_t n_recent, int32_t* kept,
+                           float* const* k_out_ptrs, float* const* v_out_ptrs,
+                           float* const* weight_out_ptrs, int64_t weight_out_stride, int32_t batch,
+                           int32_t n_kv_heads, int32_t head_dim, int64_t kv_stride);
+int32_t gla_kv_evict_f16kv(gla_ctx* ctx, uint16_t* const* k_ptrs, uint16_t* const* v_ptrs,
+                           float* const* weight_ptrs, int64_t weight_stride, const int32_t* n_pos,
+                           int32_t max_n_pos, int32_t n_keep, int32_t n_recent, int32_t* kept,
+                           uint16_t* const* k_out_ptrs, uint16_t* const* v_out_ptrs,
+                           float* const* weight_out_ptrs, int64_t weight_out_stride, int32_t batch,
+                           int32_t n_kv_heads, int32_t head_dim, int64_t kv_stride);
+
+/* ------------------------------------------------------------------------ */
 /* Introspection used by the host tests (no device work)                     */
 /* ------------------------------------------------------------------------ */
 
