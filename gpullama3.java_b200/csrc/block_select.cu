@@ -7,16 +7,28 @@
 // and the last n_last blocks are always chosen; of the others the highest
 // scores, ties to the lowest block.
 //
-// Scores are summed in FP64: which of two blocks is chosen is a comparison of
-// two sums of up to 256 products, and with FP32 sums it would depend on the
-// order of the additions (on the kernel's shape) about once in a hundred
-// selections.  An FP32 query times an FP16 or FP32 bound is exact in FP64 (48
-// bits), so what is left is 2^-53 of the sum.
+// The order is that of the sums in FP64: which of two blocks is chosen must
+// not depend on the order of additions, so on the kernel's shape.  But FP64
+// sums of everything would cost more than reading the bounds (a conversion
+// and an FMA at 1/8 and 1/2 of the FP32 rate), and few comparisons need them:
+//  1. scores in FP32.  A sum of at most 8 FMAs and 5 tree additions is within
+//     E = 2^-20 M of the exact one (13 roundings of 2^-24 of the sum of
+//     magnitudes at most); M bounds that sum for all blocks: over the lanes, a
+//     lane's largest |bound| times its sum of |coefficients|.
+//  2. the n_sel highest FP32 scores, lowest vmin, against the others, highest
+//     vmax.  If vmin - vmax > 2E the order is settled.
+//  3. otherwise scores above vmax + 2E are surely chosen (they exceed every one
+//     that was not), those below vmin - 2E surely not, and the few between are
+//     summed again in FP64 (an FP32 query times an FP16 or FP32 bound is exact
+//     there up to 2^-53) and ranked by that.
+// M = 0 (a zero query, zero bounds) means that the FP32 scores are exact; a
+// bound or query too large for E to be finite leaves everything to step 3.
 //
-// A cluster of S CTAs works on one (sequence, kv head): CTA r scores a
-// contiguous range of blocks into its shared memory, then the cluster finds
-// the n_sel-th largest key together (cache_ops.cuh) and writes the ids in
-// ascending order.  One launch, no global workspace.
+// A cluster of S CTAs works on one (sequence, kv head): each scores a
+// contiguous range of blocks and stores the keys into rank 0's shared memory,
+// where rank 0 selects alone with block barriers (a radix pass that every CTA
+// of the cluster took part in cost a cluster barrier of about 0.5 us each).
+// One launch, no global workspace.
 #include "cache_ops.cuh"
 
 namespace gla {
@@ -25,13 +37,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr float kErr = 9.5367431640625e-07f;  // 2^-20
+constexpr int kNear = 64;  // scores near the border that are ranked by comparing all pairs
 
 // Sums N values (N a power of two <= 32) over LANES lanes: each halving step
 // exchanges half of the values, so the whole costs N - 1 exchanges instead of
 // N log2(LANES).  Afterwards lane l of the group holds the sum of value
 // l >> (log2 LANES - log2 N) (lanes that share a value all hold it).
 template <int N, int LANES>
-__device__ __forceinline__ double reduce_scatter(double (&v)[N], int lane) {
+__device__ __forceinline__ float reduce_scatter(float (&v)[N], int lane) {
   int n = N;
 #pragma unroll
   for (int m = LANES / 2; m > 0; m >>= 1) {
@@ -41,8 +55,8 @@ __device__ __forceinline__ double reduce_scatter(double (&v)[N], int lane) {
 #pragma unroll
       for (int i = 0; i < N / 2; ++i) {
         if (i < n) {
-          const double keep = up ? v[i + n] : v[i];
-          const double send = up ? v[i] : v[i + n];
+          const float keep = up ? v[i + n] : v[i];
+          const float send = up ? v[i] : v[i + n];
           v[i] = keep + __shfl_xor_sync(0xffffffffu, send, m);
         }
       }
@@ -55,114 +69,311 @@ __device__ __forceinline__ double reduce_scatter(double (&v)[N], int lane) {
 
 constexpr int ilog2(int x) { return x <= 1 ? 0 : 1 + ilog2(x >> 1); }
 
+// The coefficient of a bound: min(q, 0) of lo, max(q, 0) of hi, written so
+// that a NaN stays NaN.
+__device__ __forceinline__ float coefficient(float q, bool is_lo) {
+  return is_lo ? (q > 0.f ? 0.f : q) : (q < 0.f ? 0.f : q);
+}
+
+// How a (head size, type, padded group GP) is scored.  A (block, kv head) is
+// kChunks 16-byte chunks, lo then hi, over kLanes lanes; a lane holds the
+// coefficients of its chunks in registers (at most 8 elements of GP heads) and
+// a lane group scores kBlk blocks at once, so that one reduce_scatter joins
+// them.  kBlk keeps the kernel at 128 registers: two CTAs an SM, one streams
+// while the other selects.
+template <class T, int HD, int GP>
+struct Shape {
+  static constexpr int kPer = 16 / sizeof(T);
+  static constexpr int kChunks = 2 * HD / kPer;
+  static constexpr int kLanes = kChunks > 16 ? 32 : 16;
+  static constexpr int kCpl = (kChunks + kLanes - 1) / kLanes;
+  static constexpr int kSub = 32 / kLanes;  // lane groups of a warp
+  static constexpr int kWant = GP <= 2 ? 8 / kCpl : (GP == 4 ? 4 : 4 / kCpl);
+  static constexpr int kBlk = kWant * GP > kLanes ? kLanes / GP : kWant;  // a value a lane
+  static constexpr int kVals = kBlk * GP;
+  static_assert(kCpl * kPer <= 8, "the error bound counts 8 terms a lane");
+};
+
+// The FP64 score of one (block, kv head), by one warp: the larger product of
+// each channel, so that an infinite bound on the other side does not count
+// (the FP32 scores' min(q, 0) lo + max(q, 0) hi would make it a NaN, but an
+// infinity among the bounds leaves no finite E, and all scores come here).
+template <class T, int HD>
+__device__ __forceinline__ uint64_t exact_key(const T* src, const float* s_q, int G, int lane) {
+  uint64_t key = 0;
+  for (int h = 0; h < G; ++h) {
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+      const int d = i * 32 + lane;
+      const double qd = (double)s_q[h * HD + d];
+      const double a = qd * (double)(float)src[d], c = qd * (double)(float)src[HD + d];
+      s += (a > c || a != a) ? a : c;  // a NaN of either stays
+    }
+#pragma unroll
+    for (int m = 16; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+    const uint64_t k = order_key(s);
+    key = k > key ? k : key;
+  }
+  return key;
+}
+
 // GP: heads of a group, padded to a power of two.
 template <class T, int HD, int GP>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 2)
     block_select_kernel(const float* __restrict__ q, const T* const* __restrict__ bounds_ptrs,
                         const int32_t* __restrict__ n_pos, int32_t max_n_pos,
                         int32_t* __restrict__ block_ids, int32_t n_heads, int32_t n_kv,
                         int32_t br_shift, int32_t n_sel, int32_t n_first, int32_t n_last, int S,
                         int32_t* __restrict__ status) {
-  constexpr int kPer = 16 / sizeof(T);                  // elements of a 16-byte chunk
-  constexpr int kChunks = 2 * HD / kPer;                // of one (block, head): lo then hi
-  constexpr int kLanes = kChunks >= 32 ? 32 : (kChunks > 16 ? 32 : 16);
-  constexpr int kCpl = (kChunks + kLanes - 1) / kLanes; // chunks a lane
-  constexpr int kSub = 32 / kLanes;                     // blocks side by side in a warp
-  // blocks a lane group scores at once: as many as one exchange of 32 values joins
-  constexpr int kNB = 32 / GP > 8 ? 8 : 32 / GP;
-  constexpr int kVals = kNB * GP > kLanes ? kLanes : kNB * GP;
-  constexpr int kBlk = kVals / GP;
-  extern __shared__ uint64_t s_key[];
+  using Sh = Shape<T, HD, GP>;
+  constexpr int kPer = Sh::kPer, kLanes = Sh::kLanes, kCpl = Sh::kCpl, kBlk = Sh::kBlk;
+  constexpr int kVals = Sh::kVals, kStep = kWarps * Sh::kSub * kBlk;
+  // rank 0's: one 64-bit slot a block; the FP32 keys use the low words first
+  extern __shared__ uint64_t s_slot[];
   __shared__ SelectScratch sh;
-  pdl_wait();
-  pdl_launch_dependents();
+  // rank 0's, of every warp of the cluster: M, the smallest and the largest key
+  __shared__ float s_mag[16 * kWarps];
+  __shared__ uint32_t s_min[16 * kWarps], s_max[16 * kWarps];
+  __shared__ __align__(16) float s_q[GP * HD];
+  __shared__ uint32_t s_least[kWarps], s_most[kWarps];
+  __shared__ int32_t s_near[kNear];
+  __shared__ uint64_t s_near_key[kNear];
+  __shared__ int32_t s_near_n, s_sure_n;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = S > 1 ? (int)(blockIdx.x % (unsigned)S) : 0;
   const int item = (int)(blockIdx.x / (unsigned)S);
   const int b = item / n_kv, g = item - b * n_kv;
   const int G = n_heads / n_kv;
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int i = tid; i < GP * HD; i += kThreads)
+    s_q[i] = i < G * HD ? __ldg(q + ((int64_t)b * n_heads + (int64_t)g * G) * HD + i) : 0.f;
   const int32_t n = clamped_rows(n_pos, b, max_n_pos, status);
   const T* bounds = bounds_ptrs[b];
   const bool ok = usable_ptrs(bounds, bounds, status);
   const int32_t nb = ok ? (int32_t)(((int64_t)n + (1 << br_shift) - 1) >> br_shift) : 0;
   int32_t* ids = block_ids + (int64_t)item * n_sel;
-  if (nb <= n_sel) {  // every block is chosen, whatever its score
-    for (int i = rank * kThreads + tid; i < n_sel; i += S * kThreads) ids[i] = i < nb ? i : -1;
+  // the blocks between those that are always chosen: `pick` of them
+  const int32_t pick = n_sel - n_first - n_last, nc = nb - n_first - n_last;
+  if (nb <= n_sel || pick == 0) {
+    for (int i = rank * kThreads + tid; i < n_sel; i += S * kThreads)
+      ids[i] = nb <= n_sel ? (i < nb ? i : -1) : (i < n_first ? i : nb - n_sel + i);
     return;  // every CTA of the cluster takes this way
   }
-  int32_t lo, hi;
-  share_of(nb, S, rank, &lo, &hi);
+  int32_t lo, hi;  // this CTA's candidates, counted from block n_first
+  share_of(nc, S, rank, &lo, &hi);
 
-  // this lane's coefficients: element e of its chunks, all heads
   const int sub = lane / kLanes, sl = lane % kLanes;
-  double co[kCpl * kPer][GP];
-#pragma unroll
-  for (int c = 0; c < kCpl; ++c) {
-    const int chunk = sl + c * kLanes;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-      const int el = chunk * kPer + e;  // [0, HD) lo, [HD, 2 HD) hi
-      const int d = el < HD ? el : el - HD;
-#pragma unroll
-      for (int h = 0; h < GP; ++h) {
-        float x = 0.f;
-        if (chunk < kChunks && h < G)
-          x = q[((int64_t)b * n_heads + (int64_t)g * G + h) * HD + d];
-        // a NaN query element stays NaN: its block ranks lowest
-        co[c * kPer + e][h] = (double)(el < HD ? (x > 0.f ? 0.f : x) : (x < 0.f ? 0.f : x));
-      }
-    }
-  }
   const int64_t row = (int64_t)n_kv * 2 * HD;
-  for (int32_t j0 = lo + (warp * kSub + sub) * kBlk; j0 - sub * kBlk < hi;
-       j0 += kWarps * kSub * kBlk) {
-    float4 x[kBlk][kCpl];
+  const T* base = bounds + (int64_t)n_first * row + (int64_t)g * 2 * HD;
+  float4 x[kBlk][kCpl];
+  auto load = [&](int32_t j0) {
 #pragma unroll
     for (int i = 0; i < kBlk; ++i) {
-      const T* src = bounds + (int64_t)min(j0 + i, hi - 1) * row + (int64_t)g * 2 * HD;
+      const T* src = base + (int64_t)min(j0 + i, hi - 1) * row;
 #pragma unroll
       for (int c = 0; c < kCpl; ++c) {
         const int chunk = sl + c * kLanes;
         x[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (chunk < kChunks) x[i][c] = __ldg(reinterpret_cast<const float4*>(src) + chunk);
+        if (chunk < Sh::kChunks) x[i][c] = __ldg(reinterpret_cast<const float4*>(src) + chunk);
       }
     }
-    double acc[kVals];
+  };
+  const int32_t w0 = lo + warp * Sh::kSub * kBlk;  // the warp's first block
+  if (w0 < hi) load(w0 + sub * kBlk);  // in flight while the coefficients are set up
+  cluster_arrive(S);
+  __syncthreads();
+  float co[kCpl * kPer][GP];
+#pragma unroll
+  for (int c = 0; c < kCpl; ++c) {
+    const int el = (sl + c * kLanes) * kPer;  // [0, HD) lo, [HD, 2 HD) hi
+    const int d = el < HD ? el : el - HD;
+#pragma unroll
+    for (int h = 0; h < GP; ++h)
+#pragma unroll
+      for (int p = 0; p < kPer; ++p)
+        co[c * kPer + p][h] = el < 2 * HD ? coefficient(s_q[h * HD + d + p], el < HD) : 0.f;
+  }
+
+  // keys, M and the keys' range go to rank 0's shared memory
+  uint32_t* key0 = reinterpret_cast<uint32_t*>(
+      S > 1 ? const_cast<uint64_t*>(cluster_peer(s_slot, 0)) : s_slot);
+  cluster_wait(S);  // rank 0 is running: its shared memory may be written
+  float big = 0.f;
+  bool strange = false;  // a NaN bound, which a maximum would drop
+  uint32_t kmin = ~0u, kmax = 0;
+  for (int32_t jw = w0; jw < hi; jw += kStep) {
+    const int32_t j0 = jw + sub * kBlk;
+    float acc[kVals];
 #pragma unroll
     for (int i = 0; i < kBlk; ++i) {
 #pragma unroll
-      for (int h = 0; h < GP; ++h) acc[i * GP + h] = 0.0;
+      for (int h = 0; h < GP; ++h) acc[i * GP + h] = 0.f;
 #pragma unroll
       for (int c = 0; c < kCpl; ++c) {
-        const T* e = reinterpret_cast<const T*>(&x[i][c]);
 #pragma unroll
         for (int p = 0; p < kPer; ++p) {
-          const double y = (double)(float)e[p];
+          const float y = (float)reinterpret_cast<const T*>(&x[i][c])[p];
+          big = fmaxf(big, fabsf(y));
+          strange |= y != y;
 #pragma unroll
           for (int h = 0; h < GP; ++h)
-            acc[i * GP + h] = fma(co[c * kPer + p][h], y, acc[i * GP + h]);
+            acc[i * GP + h] = fmaf(co[c * kPer + p][h], y, acc[i * GP + h]);
         }
       }
     }
-    double s = reduce_scatter<kVals, kLanes>(acc, sl);
+    if (jw + kStep < hi) load(j0 + kStep);
+    const float s = reduce_scatter<kVals, kLanes>(acc, sl);
     // lane sl holds value sl >> kRep: block value / GP, head value % GP
     constexpr int kRep = ilog2(kLanes) - ilog2(kVals);
     const int val = sl >> kRep;
     const int h = val % GP;
-    uint64_t key = h < G ? order_key(s) : 0;
+    uint32_t key = h < G ? order_key(s) : 0;
 #pragma unroll
-    for (int m = (GP << kRep) >> 1; m >= (1 << kRep) && m > 0; m >>= 1) {
-      const uint64_t o = __shfl_xor_sync(0xffffffffu, key, m);
-      key = o > key ? o : key;
-    }
+    for (int m = (GP << kRep) >> 1; m >= (1 << kRep) && m > 0; m >>= 1)
+      key = max(key, __shfl_xor_sync(0xffffffffu, key, m));
     const int32_t j = j0 + val / GP;
-    if (h == 0 && (sl & ((1 << kRep) - 1)) == 0 && j < hi)
-      s_key[j - lo] = (j < n_first || j >= nb - n_last) ? ~0ull : key;
+    if (j < hi) {
+      kmin = min(kmin, key);
+      kmax = max(kmax, key);
+      if (h == 0 && (sl & ((1 << kRep) - 1)) == 0) key0[2 * (int64_t)j] = key;
+    }
+  }
+  // M of this warp's blocks (its lane groups see different blocks: their maximum counts)
+  if (strange) big = INFINITY;
+#pragma unroll
+  for (int m = kLanes; m < 32; m <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, m));
+  float mag = 0.f;
+  bool nan_q = false;
+#pragma unroll
+  for (int h = 0; h < GP; ++h) {
+    float cs = 0.f;
+#pragma unroll
+    for (int e = 0; e < kCpl * kPer; ++e) cs += fabsf(co[e][h]);
+    cs = cs == 0.f ? 0.f : cs * big;  // an infinite bound that no coefficient meets
+#pragma unroll
+    for (int m = kLanes / 2; m > 0; m >>= 1) cs += __shfl_xor_sync(0xffffffffu, cs, m);
+    nan_q |= cs != cs;
+    mag = fmaxf(mag, cs);
+  }
+  if (nan_q || __any_sync(0xffffffffu, big == INFINITY)) mag = INFINITY;
+  kmin = __reduce_min_sync(0xffffffffu, kmin);
+  kmax = __reduce_max_sync(0xffffffffu, kmax);
+  if (lane == 0) {
+    float* mag0 = S > 1 ? const_cast<float*>(cluster_peer(s_mag, 0)) : s_mag;
+    uint32_t* min0 = S > 1 ? const_cast<uint32_t*>(cluster_peer(s_min, 0)) : s_min;
+    uint32_t* max0 = S > 1 ? const_cast<uint32_t*>(cluster_peer(s_max, 0)) : s_max;
+    mag0[rank * kWarps + warp] = mag;
+    min0[rank * kWarps + warp] = kmin;
+    max0[rank * kWarps + warp] = kmax;
+  }
+  if (tid == 0) s_near_n = s_sure_n = 0;
+  cluster_barrier(S);
+  if (rank != 0) return;
+
+  // rank 0: all keys are here
+  for (int i = tid; i < n_first + n_last; i += kThreads)
+    ids[i < n_first ? i : pick + i] = i < n_first ? i : nc + i;
+  ids += n_first;
+  uint32_t* key32 = reinterpret_cast<uint32_t*>(s_slot);
+  auto key_of = [&](int32_t i) { return key32[2 * (int64_t)i]; };
+  auto emit = [&](int32_t i, uint32_t at) { ids[at] = n_first + i; };
+  mag = 0.f;
+  kmin = ~0u;
+  kmax = 0;
+  for (int i = lane; i < S * kWarps; i += 32) {
+    mag = fmaxf(mag, s_mag[i]);
+    kmin = min(kmin, s_min[i]);
+    kmax = max(kmax, s_max[i]);
+  }
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, m));
+  kmin = __reduce_min_sync(0xffffffffu, kmin);
+  kmax = __reduce_max_sync(0xffffffffu, kmax);
+  const int bits = 32 - __clz((int)(kmax - kmin));
+  const Threshold<uint32_t> th = find_threshold<kThreads, uint32_t>(
+      sh, 1, nc, (uint32_t)pick, kmin, bits > 8 ? bits - 8 : 0, key_of);
+  // the lowest chosen and the highest other key
+  uint32_t least = ~0u, most = 0;
+#pragma unroll 4
+  for (int32_t i = tid; i < nc; i += kThreads) {
+    const uint32_t key = key_of(i);
+    if (key >= th.lo) least = min(least, key);
+    if (key < th.lo || (!th.whole && th.at(key))) most = max(most, key);
+  }
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (lane == 0) {
+    s_least[warp] = least;
+    s_most[warp] = most;
   }
   __syncthreads();
-  cluster_select<kThreads, uint64_t>(
-      sh, S, rank, hi - lo, (uint32_t)n_sel, [&](int32_t i) { return s_key[i]; },
-      [&](int32_t i, uint32_t at) { ids[at] = lo + i; });
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    least = min(least, s_least[w]);
+    most = max(most, s_most[w]);
+  }
+  // 2E, rounded up (products below FP32's normal range lose at most 2^-149 each);
+  // no bound where a sum could have overflowed
+  float two_e = mag == 0.f ? 0.f : 2.01f * kErr * mag + 1e-41f;
+  if (!(mag < 1e37f)) two_e = INFINITY;
+  const float vmin = key_score(least), vmax = key_score(most);
+  if (two_e == 0.f || vmin - vmax > two_e) {
+    emit_chosen<kThreads, uint32_t>(sh, 1, 0, nc, th, key_of, emit);
+    return;
+  }
+  // Scores too near the border for FP32.  Few: rank them among themselves.
+  for (int32_t i = tid; i < nc; i += kThreads) {
+    const float s = key_score(key_of(i));
+    if (s - vmax > two_e) {
+      atomicAdd(&s_sure_n, 1);
+    } else if (!(vmin - s > two_e)) {
+      const int32_t at = atomicAdd(&s_near_n, 1);
+      if (at < kNear) s_near[at] = i;
+    }
+  }
+  __syncthreads();
+  const int32_t near_n = s_near_n, wanted = pick - s_sure_n;
+  if (near_n <= kNear) {
+    for (int32_t i = warp; i < near_n; i += kWarps) {
+      const uint64_t k = exact_key<T, HD>(base + (int64_t)s_near[i] * row, s_q, G, lane);
+      if (lane == 0) s_near_key[i] = k;
+    }
+    __syncthreads();
+    if (tid < near_n) {
+      const uint64_t k = s_near_key[tid];
+      const int32_t me = s_near[tid];
+      int32_t before = 0;
+      for (int32_t i = 0; i < near_n; ++i)
+        before += s_near_key[i] > k || (s_near_key[i] == k && s_near[i] < me);
+      key32[2 * (int64_t)me] = before < wanted ? ~0u : 0u;
+    }
+    __syncthreads();
+    // sure ones exceed `most`; the near ones no longer do unless they are wanted
+    const Threshold<uint32_t> past{most, 0u, 0u, false};
+    emit_chosen<kThreads, uint32_t>(sh, 1, 0, nc, past, key_of, emit);
+    return;
+  }
+  // Many (equal scores, infinities): 64-bit keys for all.
+  for (int32_t i = warp; i < nc; i += kWarps) {
+    const float s = key_score(key_of(i));
+    uint64_t key64;
+    if (s - vmax > two_e) {
+      key64 = ~0ull;
+    } else if (vmin - s > two_e) {
+      key64 = 0;
+    } else {
+      key64 = exact_key<T, HD>(base + (int64_t)i * row, s_q, G, lane);
+    }
+    __syncwarp();
+    if (lane == 0) s_slot[i] = key64;
+  }
+  __syncthreads();
+  auto slot_of = [&](int32_t i) { return s_slot[i]; };
+  const Threshold<uint64_t> th64 = find_threshold<kThreads, uint64_t>(
+      sh, 1, nc, (uint32_t)pick, (uint64_t)0, 56, slot_of);
+  emit_chosen<kThreads, uint64_t>(sh, 1, 0, nc, th64, slot_of, emit);
 }
 
 template <class T, int HD, int GP>
@@ -173,23 +384,20 @@ int launch_select(const SelectRequest& r, const DeviceInfo& dev, cudaStream_t st
   while ((1 << br_shift) < r.block_rows) ++br_shift;
   const int64_t items = (int64_t)r.batch * r.n_kv;
   const int64_t max_nb = ((int64_t)r.max_n_pos + r.block_rows - 1) / r.block_rows;
-  // as many CTAs a (sequence, kv head) as fill the device once, while each
-  // still has 64 blocks to score; and enough for the keys to fit shared memory
-  const int64_t key_cap = (dev.smem_optin - 8 * 1024) / 8;
-  int S = 1;
-  while (S < 16 && ((items * S < dev.sms && max_nb > 64 * S) || (max_nb + S - 1) / S > key_cap))
-    S *= 2;
-  const int64_t per = (max_nb + S - 1) / S;
-  if (per > key_cap) {
-    *err = "too many blocks for one selection";
+  if (max_nb > kMaxSelectBlocks) {
+    *err = "too many blocks for one selection: use larger blocks";
     return GLA_ERR_NOT_SUPPORTED;
   }
+  // as many CTAs a (sequence, kv head) as fill the device (two an SM), while each
+  // still has 64 blocks to score
+  int S = 1;
+  while (S < 16 && items * S < 2 * dev.sms && max_nb > 64 * S) S *= 2;
   if (items * S > INT32_MAX) {
     *err = "batch * n_kv_heads too large";
     return GLA_ERR_NOT_SUPPORTED;
   }
   return launch_clusters(block_select_kernel<T, HD, GP>, (unsigned)(items * S), kThreads,
-                         (size_t)per * 8, S, attr_done, stream, "block selection", err, r.q,
+                         (size_t)max_nb * 8, S, attr_done, stream, "block selection", err, r.q,
                          reinterpret_cast<const T* const*>(r.bounds_ptrs), r.n_pos, r.max_n_pos,
                          r.block_ids, r.n_heads, r.n_kv, br_shift, r.n_sel, r.n_first, r.n_last, S,
                          r.status);

@@ -57,6 +57,14 @@ __device__ __forceinline__ void cluster_barrier(int S) {
   }
 }
 
+// The same barrier in two halves, for work between them; a cluster of one passes.
+__device__ __forceinline__ void cluster_arrive(int S) {
+  if (S > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait(int S) {
+  if (S > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Address, in CTA `rank` of the cluster, of the shared memory object `p` of this CTA.
 template <class T>
 __device__ __forceinline__ const T* cluster_peer(const T* p, int rank) {
@@ -127,56 +135,69 @@ __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t u = __float_as_uint(__fadd_rn(x, 0.0f));
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
+// The score of an FP32 key; keys that are no score's are the infinities.
+__device__ __forceinline__ float key_score(uint32_t key) {
+  if (key == 0) return -INFINITY;
+  if (key == ~0u) return INFINITY;
+  return __uint_as_float((key >> 31) ? (key & 0x7fffffffu) : ~key);
+}
 
 // ---------------------------------------------------------------------------
 // The k largest of the keys that the CTAs of a cluster hold together, ties to
 // the lowest index.  CTA r holds the n_local keys key(0..n_local-1) of a
 // contiguous index range, ranges ascending with the rank; 0 < k < all keys.
+// The keys are walked once a pass: they belong in shared memory.
 //
-// Radix selection, 8 bits a pass from the top: every CTA counts the digits of
-// its keys that match the prefix found so far, one cluster barrier publishes
-// the counts, and every CTA adds all ranks' counts itself (so the ranks agree
+// find_threshold: radix selection, 8 bits a pass.  Every CTA counts the digits
+// of its keys in the range found so far, one cluster barrier publishes the
+// counts, and every CTA adds all ranks' counts itself (so the ranks agree
 // without a second barrier; two count buffers keep a fast rank from clearing
 // what a slow one still reads).  A pass whose bin is taken whole ends the
-// search.  A second walk writes the chosen indices in ascending order:
+// search.  The first range, [base, base + 256 << shift), holds every key; a
+// caller that knows the smallest and largest key passes a range that fits
+// them: full-width digits would put nearly all scores into a few bins first.
+// emit_chosen: each warp, which owns a contiguous share of the CTA's keys,
+// counts what it holds above and at the threshold, and after one more barrier
+// writes its chosen indices, so the list ascends with no barrier inside:
 // emit(local index, position in the list of all chosen).
 // ---------------------------------------------------------------------------
+constexpr int kSelectWarps = 16;  // at most
 struct SelectScratch {
   uint32_t hist[2][256];
-  uint32_t warp_sum[32];
-  uint32_t warp_sum2[32];
-  uint32_t found[3];       // digit, keys above it, keys in it
-  uint32_t counts[2];      // this CTA's keys above / at the threshold
+  uint32_t warp_sum[8];
+  uint32_t found[3];                 // digit, keys above it, keys in it
+  uint32_t above[kSelectWarps];      // of each warp's share: keys above the threshold
+  uint32_t at[kSelectWarps];         // and at it
+  uint32_t counts[2];                // of the CTA's share
 };
 
-template <int THREADS, class Key, class KeyFn, class Emit>
-__device__ __forceinline__ void cluster_select(SelectScratch& sh, int S, int rank, int32_t n_local,
-                                               uint32_t k, KeyFn key, Emit emit) {
+template <class Key>
+struct Threshold {
+  Key lo, span;      // chosen: keys above lo + span, and of those in [lo, lo + span] ...
+  uint32_t need;     // ... the first `need`
+  bool whole;        // which are all of them
+  __device__ __forceinline__ bool at(Key k) const { return k >= lo && k - lo <= span; }
+  __device__ __forceinline__ bool above(Key k) const { return k >= lo && k - lo > span; }
+};
+
+template <int THREADS, class Key, class KeyFn>
+__device__ __forceinline__ Threshold<Key> find_threshold(SelectScratch& sh, int S, int32_t n_local,
+                                                         uint32_t k, Key base, int shift,
+                                                         KeyFn key) {
   static_assert(THREADS >= 256 && THREADS % 32 == 0, "one thread per histogram bin");
-  constexpr int kBits = sizeof(Key) * 8;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  Key prefix = 0, mask = 0;
-  uint32_t need = k;  // of the keys that match the prefix
+  uint32_t need = k;  // of the keys in the range
   bool whole = false;
   int buf = 0;
-  for (int shift = kBits - 8; shift >= 0 && !whole; shift -= 8, buf ^= 1) {
-    for (int i = tid; i < 256; i += THREADS) sh.hist[buf][i] = 0;
-    __syncthreads();
-    for (int32_t i0 = 0; i0 < n_local; i0 += THREADS) {
-      const int32_t i = i0 + tid;
-      Key kv = 0;
-      bool in = i < n_local;
-      if (in) {
-        kv = key(i);
-        in = (kv & mask) == prefix;
-      }
-      const unsigned live = __ballot_sync(0xffffffffu, in);
-      if (in) {
-        // the top digits of scores are nearly all the same: one add a warp and digit
-        const uint32_t d = (uint32_t)(kv >> shift) & 255u;
-        const unsigned same = __match_any_sync(live, d);
-        if (lane == __ffs(same) - 1) atomicAdd(&sh.hist[buf][d], (uint32_t)__popc(same));
-      }
+  Key span = ~(Key)0;  // the range is [base, base + span]
+  for (int i = tid; i < 512; i += THREADS) (&sh.hist[0][0])[i] = 0;
+  __syncthreads();
+  for (;; buf ^= 1) {
+#pragma unroll 4
+    for (int32_t i = tid; i < n_local; i += THREADS) {
+      const Key kv = key(i);
+      if (kv >= base && kv - base <= span)
+        atomicAdd(&sh.hist[buf][(uint32_t)((kv - base) >> shift) & 255u], 1u);
     }
     cluster_barrier(S);
     uint32_t mine = 0;
@@ -184,8 +205,10 @@ __device__ __forceinline__ void cluster_select(SelectScratch& sh, int S, int ran
       if (S == 1) {
         mine = sh.hist[buf][255 - tid];
       } else {
+#pragma unroll 4
         for (int r = 0; r < S; ++r) mine += *cluster_peer(&sh.hist[buf][255 - tid], r);
       }
+      sh.hist[buf ^ 1][tid] = 0;  // every rank has read it: it did so before the barrier
     }
     // thread t holds bin 255 - t: the inclusive scan counts the keys at or above it
     uint32_t inc = mine;
@@ -194,10 +217,11 @@ __device__ __forceinline__ void cluster_select(SelectScratch& sh, int S, int ran
       const uint32_t x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    if (lane == 31) sh.warp_sum[warp] = inc;
+    if (tid < 256 && lane == 31) sh.warp_sum[warp] = inc;
     __syncthreads();
     if (tid < 256) {
-      for (int w = 0; w < warp; ++w) inc += sh.warp_sum[w];
+#pragma unroll
+      for (int w = 0; w < 7; ++w) inc += w < warp ? sh.warp_sum[w] : 0;
       if (inc - mine < need && need <= inc) {
         sh.found[0] = 255 - tid;
         sh.found[1] = inc - mine;
@@ -207,71 +231,78 @@ __device__ __forceinline__ void cluster_select(SelectScratch& sh, int S, int ran
     __syncthreads();
     need -= sh.found[1];
     whole = sh.found[2] == need;
-    prefix |= (Key)sh.found[0] << shift;
-    mask |= (Key)255 << shift;
+    base += (Key)sh.found[0] << shift;
+    span = ((Key)1 << shift) - 1;
+    if (whole || shift == 0) break;
+    shift = shift > 8 ? shift - 8 : 0;
   }
-  // chosen: above the prefix, or at it (all of those if `whole`, else the first `need`)
+  return Threshold<Key>{base, span, need, whole};
+}
+
+template <int THREADS, class Key, class KeyFn, class Emit>
+__device__ __forceinline__ void emit_chosen(SelectScratch& sh, int S, int rank, int32_t n_local,
+                                            const Threshold<Key>& th, KeyFn key, Emit emit) {
+  constexpr int W = THREADS / 32;
+  static_assert(W <= kSelectWarps, "per-warp counts");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t need = th.need;
+  // this warp's share of the CTA's keys: whole warps of them, contiguous
+  const int32_t share = ((n_local + THREADS - 1) / THREADS) * 32;
+  const int32_t w_lo = min(warp * share, n_local), w_hi = min(w_lo + share, n_local);
   uint32_t above = 0, at = 0;
-  for (int32_t i = tid; i < n_local; i += THREADS) {
-    const Key kv = key(i) & mask;
-    above += kv > prefix;
-    at += kv == prefix;
+#pragma unroll 4
+  for (int32_t i = w_lo + lane; i < w_hi; i += 32) {
+    const Key kv = key(i);
+    above += th.above(kv);
+    at += th.at(kv);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    above += __shfl_xor_sync(0xffffffffu, above, o);
-    at += __shfl_xor_sync(0xffffffffu, at, o);
-  }
+  above = __reduce_add_sync(0xffffffffu, above);
+  at = __reduce_add_sync(0xffffffffu, at);
   if (lane == 0) {
-    sh.warp_sum[warp] = above;
-    sh.warp_sum2[warp] = at;
+    sh.above[warp] = above;
+    sh.at[warp] = at;
   }
   __syncthreads();
-  if (tid == 0) {
-    uint32_t a = 0, e = 0;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      a += sh.warp_sum[w];
-      e += sh.warp_sum2[w];
+  if (S > 1) {
+    if (tid == 0) {
+      uint32_t a = 0, e = 0;
+      for (int w = 0; w < W; ++w) {
+        a += sh.above[w];
+        e += sh.at[w];
+      }
+      sh.counts[0] = a;
+      sh.counts[1] = e;
     }
-    sh.counts[0] = a;
-    sh.counts[1] = e;
+    cluster_barrier(S);
   }
-  cluster_barrier(S);
+  // keys chosen, and keys at the threshold, before this warp's share
   uint32_t out = 0, at_before = 0;
-  for (int r = 0; r < rank; ++r) {
-    const uint32_t* c = S == 1 ? sh.counts : cluster_peer(sh.counts, r);
-    const uint32_t a = c[0], e = c[1];
+  auto skip = [&](uint32_t a, uint32_t e) {
     const uint32_t room = need > at_before ? need - at_before : 0;
     out += a + (e < room ? e : room);
     at_before += e;
-  }
-  for (int32_t i0 = 0; i0 < n_local; i0 += THREADS) {
-    const int32_t i = i0 + tid;
-    Key kv = 0;
-    if (i < n_local) kv = key(i) & mask;
-    const bool gt = i < n_local && kv > prefix, eq = i < n_local && kv == prefix;
+  };
+  if (S > 1)
+    for (int r = 0; r < rank; ++r) {
+      const uint32_t* c = cluster_peer(sh.counts, r);
+      skip(c[0], c[1]);
+    }
+#pragma unroll
+  for (int w = 0; w < W - 1; ++w)
+    if (w < warp) skip(sh.above[w], sh.at[w]);
+  const unsigned below = (1u << lane) - 1;
+#pragma unroll 4
+  for (int32_t i0 = w_lo; i0 < w_hi; i0 += 32) {
+    const int32_t i = i0 + lane;
+    const bool in = i < w_hi;
+    const Key kv = key(in ? i : w_lo);
+    const bool eq = in && th.at(kv);
     const unsigned beq = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) sh.warp_sum2[warp] = __popc(beq);
-    __syncthreads();
-    uint32_t eq_pos = at_before + __popc(beq & ((1u << lane) - 1)), eq_all = 0;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      const uint32_t x = sh.warp_sum2[w];
-      if (w < warp) eq_pos += x;
-      eq_all += x;
-    }
-    const bool take = gt || (eq && eq_pos < need);
+    const bool take = (in && th.above(kv)) || (eq && at_before + __popc(beq & below) < need);
     const unsigned bt = __ballot_sync(0xffffffffu, take);
-    if (lane == 0) sh.warp_sum[warp] = __popc(bt);
-    __syncthreads();
-    uint32_t pos = out + __popc(bt & ((1u << lane) - 1)), all = 0;
-    for (int w = 0; w < THREADS / 32; ++w) {
-      const uint32_t x = sh.warp_sum[w];
-      if (w < warp) pos += x;
-      all += x;
-    }
-    if (take) emit(i, pos);
-    out += all;
-    at_before += eq_all;
+    if (take) emit(i, out + __popc(bt & below));
+    out += __popc(bt);
+    at_before += __popc(beq);
   }
   cluster_barrier(S);  // no CTA leaves while another still reads its counts
 }

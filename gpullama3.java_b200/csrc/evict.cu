@@ -25,7 +25,8 @@ __global__ void __launch_bounds__(kSelThreads)
     evict_select_kernel(const float* const* __restrict__ weight_ptrs, int64_t weight_stride,
                         const int32_t* __restrict__ n_pos, int32_t max_n_pos, int32_t n_keep,
                         int32_t n_recent, int32_t* __restrict__ kept, int32_t n_kv, int S,
-                        int32_t* __restrict__ status) {
+                        int32_t key_cap, int32_t* __restrict__ status) {
+  extern __shared__ uint32_t s_key[];
   __shared__ SelectScratch sh;
   pdl_wait();
   pdl_launch_dependents();
@@ -49,9 +50,15 @@ __global__ void __launch_bounds__(kSelThreads)
   int32_t lo, hi;
   share_of(older, S, rank, &lo, &hi);
   const float* mine = w + (int64_t)g * weight_stride + lo;
-  cluster_select<kSelThreads, uint32_t>(
-      sh, S, rank, hi - lo, (uint32_t)pick, [&](int32_t i) { return order_key(mine[i]); },
-      [&](int32_t i, uint32_t at) { out[at] = lo + i; });
+  const int32_t staged = min(hi - lo, key_cap);
+#pragma unroll 8
+  for (int32_t i = tid; i < staged; i += kSelThreads) s_key[i] = order_key(__ldcg(mine + i));
+  __syncthreads();
+  auto key = [&](int32_t i) { return i < staged ? s_key[i] : order_key(__ldcg(mine + i)); };
+  const Threshold<uint32_t> th =
+      find_threshold<kSelThreads, uint32_t>(sh, S, hi - lo, (uint32_t)pick, 0u, 24, key);
+  emit_chosen<kSelThreads, uint32_t>(sh, S, rank, hi - lo, th, key,
+                                     [&](int32_t i, uint32_t at) { out[at] = lo + i; });
 }
 
 // Kept rows of one kv head to another cache: thread = (row, 16-byte chunk).
@@ -262,17 +269,24 @@ int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stre
                  std::string* err) {
   static std::atomic<uint64_t> attr_done{0};
   const int64_t items = (int64_t)r.batch * r.n_kv;
-  // a CTA for every 2048 weights, as long as that does not exceed the device
+  // a CTA for every 2048 weights, as long as that does not exceed the device; and
+  // enough for the keys to fit shared memory (past 16 CTAs the rest is read again a pass)
+  const int64_t most_keys = (dev.smem_optin - 8 * 1024) / 4;
   int S = 1;
-  while (S < 16 && items * S < dev.sms && r.max_n_pos > (int64_t)2048 * S) S *= 2;
+  while (S < 16 && ((items * S < dev.sms && r.max_n_pos > (int64_t)2048 * S) ||
+                    r.max_n_pos > most_keys * S))
+    S *= 2;
+  const int32_t key_cap =
+      (int32_t)std::min<int64_t>(most_keys, ((int64_t)r.max_n_pos + S - 1) / S);
   if (items * S > INT32_MAX) {
     *err = "batch * n_kv_heads too large";
     return GLA_ERR_NOT_SUPPORTED;
   }
-  int rc = launch_clusters(evict_select_kernel, (unsigned)(items * S), kSelThreads, 0, S, attr_done,
+  int rc = launch_clusters(evict_select_kernel, (unsigned)(items * S), kSelThreads,
+                           (size_t)key_cap * 4, S, attr_done,
                            stream, "evict selection", err,
                            (const float* const*)r.weight_ptrs, r.weight_stride, r.n_pos,
-                           r.max_n_pos, r.n_keep, r.n_recent, r.kept, r.n_kv, S, r.status);
+                           r.max_n_pos, r.n_keep, r.n_recent, r.kept, r.n_kv, S, key_cap, r.status);
   if (rc != GLA_OK) return rc;
   return r.dtype == GLA_DTYPE_F16 ? move_dim<__half>(r, stream, err)
                                   : move_dim<float>(r, stream, err);

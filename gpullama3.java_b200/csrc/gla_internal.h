@@ -168,6 +168,8 @@ struct AppendRequest {  // append_batched.cu
 };
 int launch_append_batched(const AppendRequest& r, cudaStream_t stream, std::string* err);
 
+// Most blocks of one selection: their keys lie in one CTA's shared memory.
+constexpr int32_t kMaxSelectBlocks = 24576;
 struct SelectRequest {  // block_select.cu
   int dtype;
   const float* q;

@@ -553,12 +553,12 @@ int32_t gla_rope_append_batched_f16kv(gla_ctx* ctx, const float* q, const float*
  * [n_sel] (DEVICE int32), ascending, -1 behind the last one.  Of the n_blocks =
  * ceil(n_pos / block_rows) blocks the first n_first and the last n_last are always
  * chosen (n_first + n_last <= n_sel), the others by
- *     score(j, g) = max over the q heads h of g of
- *                   sum_d (min(q_hd, 0) lo_jgd + max(q_hd, 0) hi_jgd),
- * an upper bound of q_h . k_t over block j's rows (for a positive scale), summed in
- * FP64; the highest are chosen, ties to the lowest block, a head whose sum is NaN (an
- * infinite bound times zero is) counts as the lowest.  With n_blocks <= n_sel all are
- * chosen.  Batch entries may share bounds: the queries of
+ *     score(j, g) = max over the q heads h of g of sum_d max(q_hd lo_jgd, q_hd hi_jgd),
+ * an upper bound of q_h . k_t over block j's rows (for a positive scale; lo <= hi, as
+ * gla_block_bounds_* gives them).  The order is that of the sums in FP64: the highest
+ * are chosen, ties to the lowest block, a head whose sum is NaN counts as the lowest.  With n_blocks <= n_sel all are
+ * chosen.  max_n_pos / block_rows, rounded up, at most 24576 (else
+ * GLA_ERR_NOT_SUPPORTED).  Batch entries may share bounds: the queries of
  * a prompt chunk over one cache, each with its own n_pos and blocks. */
 int32_t gla_block_select_f32kv(gla_ctx* ctx, const float* q, const float* const* bounds_ptrs,
                                const int32_t* n_pos, int32_t max_n_pos, int32_t* block_ids,

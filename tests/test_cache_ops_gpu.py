@@ -788,3 +788,78 @@ def test_refusals(gla_ctx):
     refuse(-1, c.rope_append_batched, **app(style=2))
     refuse(-1, c.rope_append_batched, **app(context_length=0))
     assert c.device_status() == 0
+
+
+# ------------------------------------------------------------------------- near the border
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("nh,n_kv,hd", [(8, 2, 64), (7, 1, 128), (3, 3, 96), (4, 2, 128)])
+def test_select_decides_below_fp32_rounding(gla_ctx, t, nh, n_kv, hd):
+    """Scores that differ by less than an FP32 sum's rounding, by nothing, and by much:
+    the order is that of the 64-bit sums.  Whole-number bounds and queries of 2^-30 steps
+    make every 64-bit sum exact, so the reference's order is the true one."""
+    g, br, nb = rng(20, nh, hd), 16, 700
+    base = torch.randint(-3, 4, (1, n_kv, 2, hd), generator=g, device="cuda").float().sort(dim=2)[0]
+    bs = base.repeat(nb, 1, 1, 1)
+    # one channel of a block moves by one: times a query element of about 2^-20
+    at = torch.randint(0, nb, (nb,), generator=g, device="cuda")
+    bs[at, :, :, 0] += torch.randint(0, 5, (nb, 1, 1), generator=g, device="cuda").float()
+    bs[::97, :, :, 1:9] += 2
+    bs[5::89, :, :, 1:9] -= 3
+    q = torch.randint(-(1 << 8), 1 << 8, (1, nh, hd), generator=g, device="cuda").float() / 64
+    q[:, :, 0] = torch.randint(1, 1 << 10, (1, nh), generator=g, device="cuda").float() * 2.0 ** -30
+    bs = bs.to(DT[t]).contiguous()
+    for n_sel, first, last in ((1, 0, 0), (11, 1, 2), (350, 0, 1), (690, 0, 0)):
+        ids = torch.empty(1, n_kv, n_sel, dtype=torch.int32, device="cuda")
+        gla_ctx.block_select(q, ptrs([bs]), i32([nb * br]), nb * br, ids, 1, nh, n_kv, hd, br, n_sel,
+                             n_first=first, n_last=last, f16_cache=t == "f16")
+        ok(gla_ctx)
+        want, _ = select64(q[0], bs, nb * br, br, n_sel, first, last)
+        np.testing.assert_array_equal(ids[0].cpu().numpy(), want)
+
+
+def test_select_magnitudes(gla_ctx):
+    """FP32 sums that overflow, queries of NaN, infinity and zero, tiny products."""
+    g, nh, n_kv, hd, br, nb, n_sel = rng(21), 2, 1, 64, 16, 200, 9
+    b0 = normal(g, nb, n_kv, 2, hd).sort(dim=2)[0]
+    q0 = normal(g, 1, nh, hd)
+    cases = [(b0 * 1e30, q0 * 1e8), (b0 * 1e-30, q0 * 1e-12), (b0, q0 * 0), (b0 * 0, q0),
+             (b0 * 3e38 / 8, q0 / 4)]
+    for bo, q in cases:
+        bo, q = bo.contiguous(), q.contiguous()
+        ids = torch.empty(1, n_kv, n_sel, dtype=torch.int32, device="cuda")
+        gla_ctx.block_select(q, ptrs([bo]), i32([nb * br]), nb * br, ids, 1, nh, n_kv, hd, br, n_sel,
+                             n_last=0)
+        ok(gla_ctx)
+        want, _ = select64(q[0], bo, nb * br, br, n_sel, 0, 0)
+        np.testing.assert_array_equal(ids[0].cpu().numpy(), want)
+    q = q0.clone()
+    q[0, 1, 3] = float("nan")  # that head counts as the lowest: the other one decides
+    ids = torch.empty(1, n_kv, n_sel, dtype=torch.int32, device="cuda")
+    gla_ctx.block_select(q, ptrs([b0]), i32([nb * br]), nb * br, ids, 1, nh, n_kv, hd, br, n_sel, n_last=0)
+    ok(gla_ctx)
+    want, _ = select64(q0[0, :1], b0, nb * br, br, n_sel, 0, 0)
+    np.testing.assert_array_equal(ids[0].cpu().numpy(), want)
+
+
+def test_select_refuses_more_blocks_than_it_holds(gla_ctx):
+    q = torch.zeros(8 * 64, device="cuda")
+    p, ids = torch.zeros(1, dtype=torch.int64, device="cuda"), i32([0] * 64)
+    with pytest.raises(gla.GlaError) as e:
+        gla_ctx.block_select(q, p, i32([0]), 24576 * 16 + 1, ids, 1, 8, 2, 64, 16, 2)
+    assert e.value.status == -3
+    gla_ctx.block_select(q, p, i32([0]), 24576 * 16, ids, 1, 8, 2, 64, 16, 2)  # a null pointer: -1s
+    assert gla_ctx.device_status() == -1 and (ids[:4] == -1).all()
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_select_over_the_most_blocks(gla_ctx, t):
+    g, nh, n_kv, hd, br, nb, n_sel = rng(22), 4, 1, 64, 16, 24576, 4000
+    bs = normal(g, nb, n_kv, 2, hd).sort(dim=2)[0].to(DT[t]).contiguous()
+    q = normal(g, 1, nh, hd)
+    ids = torch.empty(1, n_kv, n_sel, dtype=torch.int32, device="cuda")
+    gla_ctx.block_select(q, ptrs([bs]), i32([nb * br - 3]), nb * br, ids, 1, nh, n_kv, hd, br, n_sel,
+                         n_first=2, n_last=3, f16_cache=t == "f16")
+    ok(gla_ctx)
+    want, gap = select64(q[0], bs, nb * br - 3, br, n_sel, 2, 3)
+    assert gap > 1e-11
+    np.testing.assert_array_equal(ids[0].cpu().numpy(), want)
