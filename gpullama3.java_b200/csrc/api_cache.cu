@@ -45,6 +45,7 @@ int check_stride(gla_ctx* ctx, int dtype, int32_t n_kv, int32_t head_dim, int64_
     return fail(ctx, GLA_ERR_INVALID_ARG, "kv_stride must be >= n_kv_heads * head_dim");
   if (kv_stride % (dtype == GLA_DTYPE_F16 ? 8 : 4) != 0)
     return fail(ctx, GLA_ERR_ALIGNMENT, "kv_stride must be a multiple of 16 bytes");
+  if (kv_stride > (1 << 28)) return fail(ctx, GLA_ERR_NOT_SUPPORTED, "kv_stride above 2^28");
   return GLA_OK;
 }
 
@@ -267,7 +268,7 @@ int32_t decode_weights(gla_ctx* ctx, int dtype, const float* q, const void* cons
                                      n_heads, n_kv_heads, head_dim, kv_stride, scale);
     r.weight_ptrs = weight_ptrs;
     r.weight_stride = weight_stride;
-    rc = ensure_scores(ctx, attend_score_floats(r));
+    rc = ensure_scores(ctx, attend_score_floats(r, ctx->dev));
     if (rc != GLA_OK) return rc;
     r.scores = ctx->scores;
     std::string err;

@@ -203,7 +203,7 @@ struct AttendRequest {  // row_attend.cu
   float* scores = nullptr;              // workspace of attend_score_floats(...) floats
   int32_t* status;
 };
-size_t attend_score_floats(const AttendRequest& r);
+size_t attend_score_floats(const AttendRequest& r, const DeviceInfo& dev);
 int launch_attend(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,
                   std::string* err);
 

@@ -15,7 +15,7 @@
 // maximum, sum and output: no block barrier inside the stream.  The warps join
 // in shared memory and the CTAs through the cluster's shared memory, in a
 // fixed order, so results do not depend on timing, and there is no workspace,
-// counter or second launch.  Rows in shared memory are padded by 16 bytes: a
+// counter or second launch (but see split_parts).  Rows in shared memory are padded by 16 bytes: a
 // row's pitch is an odd number of 16-byte chunks, which keeps ldmatrix and the
 // vector loads free of bank conflicts.
 //
@@ -26,12 +26,17 @@
 // its largest (so the low halves do not fall under FP16's range), p by 2^15
 // (p <= 1; a weight of 2^-17 still has all 22 bits).  tcgen05 has no place
 // here: 8 rows of a 128-row tile, and the stream is HBM-bound.
-// FP32 cache: FP32 pairs on the CUDA cores.
+// FP32 cache: the same with mma.sync.m16n8k8 on TF32 halves (split_tf32) of q and p
+// (the two row halves of A) and of K and V (two products).  On the CUDA cores a unit of 8 rows and 8 heads took about 600
+// instructions, this way about 330, whatever the group.
+// Rows are taken to be finite: an infinite key or value makes lo a NaN.
 //
 // Weights: the normalisation is known only when all rows were seen, so the
 // scores (log2 units) go to a workspace, G floats a row against 2 head_dim
-// elements of K and V, and each CTA reads its own rows' scores again (from L2)
-// after the cluster has joined its maxima and sums.
+// elements of K and V (read with an evict-first hint, so the scores stay in L2),
+// and are read again to add the weights.  Long sequences: the rows are cut into
+// parts of equal size, one CTA each, so that a ragged batch still fills the
+// device evenly, and a second kernel joins the parts and adds the weights.
 #include <cmath>
 
 #include "cache_ops.cuh"
@@ -40,8 +45,6 @@ namespace gla {
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPScale = 32768.0f;  // FP16 path: p enters the product times 2^15
 
@@ -51,10 +54,29 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// 16-byte cp.async that reads `bytes` (16 or 0) and zero-fills the rest.
-__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
-               : "memory");
+// 16-byte cp.async that reads `bytes` (16 or 0) and zero-fills the rest; ONCE:
+// data that is read once, first to leave L2.
+template <bool ONCE>
+__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, int bytes,
+                                                  uint64_t policy) {
+  if constexpr (ONCE) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst),
+                 "l"(src), "r"(bytes), "l"(policy)
+                 : "memory");
+  } else {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+                 : "memory");
+  }
+}
+template <bool ONCE>
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint64_t policy) {
+  if constexpr (ONCE) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst),
+                 "l"(src), "l"(policy)
+                 : "memory");
+  } else {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  }
 }
 __device__ __forceinline__ void cp_async_commit() {
   asm volatile("cp.async.commit_group;" ::: "memory");
@@ -85,6 +107,26 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void lds_f32x2(uint32_t addr, float (&v)[2]) {
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr));
+}
+
+// x = hi + lo, up to what the matrix instruction drops of lo: hi is x rounded to
+// TF32's 11 bits, so |lo| is at most 2^12 units of x's last place (2^-23 of its
+// power of two), and of its 12 bits 11 count: one unit at most is lost.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
 __device__ __forceinline__ uint32_t pack_half2(__half a, __half b) {
   const __half2 v = __halves2half2(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -97,14 +139,18 @@ struct AttendParams {
   const int32_t* n_pos;
   int32_t max_n_pos;
   float* xb;
-  int32_t n_heads, n_kv, S;
-  int64_t kv_stride;
+  int32_t n_heads, n_kv;
+  int32_t S;          // CTAs of an item: a cluster, or (part != null) parts joined later
+  uint32_t kv_bytes;  // of a cache row
   float scale_log2;  // scale * log2(e)
   const int32_t* block_ids;
   int32_t n_sel, br_shift;
   float* const* weight_ptrs;
   int64_t weight_stride;
-  float* scores;  // [batch][n_kv][max_n_pos][G]
+  float* scores;      // [item][G][score_pitch]
+  int64_t score_pitch;
+  float* part;        // [item][S][G][HD + 2]: o, then (m, l) of each head
+  int32_t part_rows;  // of a part
   int32_t* status;
 };
 
@@ -125,23 +171,34 @@ __device__ __forceinline__ int32_t unit_row(const AttendParams& p, const int32_t
   return row < n ? (int32_t)row : -1;
 }
 
-// Copies unit rows [row0, row0 + U) of K and V into a ring slot (K then V).
-template <class T, int HD, int U>
-__device__ __forceinline__ void load_unit(uint32_t slot, const T* k, const T* v, int64_t kv_stride,
-                                          int32_t row0, int32_t n, int lane) {
+// Copies unit rows [row0, row0 + U) of K and V into a ring slot (K then V);
+// rows from n on are zero-filled, not read.
+template <class T, int HD, int U, bool ONCE>
+__device__ __forceinline__ void load_unit(uint32_t slot, const T* k, const T* v, uint32_t kv_bytes,
+                                          int32_t row0, int32_t n, uint64_t policy, int lane) {
   constexpr int kChunks = HD * (int)sizeof(T) / 16;
   constexpr int kPitch = HD * (int)sizeof(T) + 16;
-  constexpr int kPer = 16 / (int)sizeof(T);
+  const char* kr = reinterpret_cast<const char*>(k) + (uint64_t)(uint32_t)row0 * kv_bytes;
+  const char* vr = reinterpret_cast<const char*>(v) + (uint64_t)(uint32_t)row0 * kv_bytes;
+  if (n - row0 >= U) {
 #pragma unroll
-  for (int i = 0; i < U * kChunks / 32; ++i) {
-    const int c = i * 32 + lane;
-    const int r = c / kChunks, ch = c - r * kChunks;
-    const int32_t row = row0 + r;
-    const int bytes = row < n ? 16 : 0;
-    const int64_t off = (int64_t)(row < n ? row : row0) * kv_stride + ch * kPer;
-    const uint32_t dst = slot + r * kPitch + ch * 16;
-    cp_async_16_zfill(dst, k + off, bytes);
-    cp_async_16_zfill(dst + U * kPitch, v + off, bytes);
+    for (int i = 0; i < U * kChunks / 32; ++i) {
+      const uint32_t c = i * 32 + lane, r = c / kChunks, ch = c - r * kChunks;
+      const uint32_t dst = slot + r * kPitch + ch * 16;
+      const uint64_t off = (uint64_t)r * kv_bytes + ch * 16;
+      cp_async_16<ONCE>(dst, kr + off, policy);
+      cp_async_16<ONCE>(dst + U * kPitch, vr + off, policy);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < U * kChunks / 32; ++i) {
+      const uint32_t c = i * 32 + lane, r = c / kChunks, ch = c - r * kChunks;
+      const int bytes = (int32_t)r < n - row0 ? 16 : 0;
+      const uint32_t dst = slot + r * kPitch + ch * 16;
+      const uint64_t off = bytes ? (uint64_t)r * kv_bytes + ch * 16 : 0;
+      cp_async_16_zfill<ONCE>(dst, kr + off, bytes, policy);
+      cp_async_16_zfill<ONCE>(dst + U * kPitch, vr + off, bytes, policy);
+    }
   }
 }
 
@@ -153,16 +210,27 @@ template <class T, int HD>
 constexpr int slot_bytes() {
   return 2 * unit_rows<T, HD>() * (HD * (int)sizeof(T) + 16);
 }
-// As deep a ring as one CTA an SM allows.
-template <class T, int HD>
-constexpr int ring_stages() {
-  return 212 * 1024 / (kWarps * slot_bytes<T, HD>());
-}
+// Two shapes of CTA.  Wide: 8 warps with a ring as deep as one CTA an SM
+// allows, for calls whose clusters do not fill the device; a warp's few units
+// are then all in flight at once.  Slim: 4 warps with rings of 72 KB in all,
+// three CTAs an SM (168 registers a thread): 12 warps hide the dependent steps
+// of a unit (product, maximum, exponential, product), which 8 warps do not, and
+// one CTA streams while another starts or joins.
+template <class T, int HD, bool WIDE>
+struct Cta {
+  static constexpr int kWarps = WIDE ? 8 : 4;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kBudget = (WIDE ? 212 : 70) * 1024;
+  static constexpr int kStages = kBudget / (kWarps * slot_bytes<T, HD>());
+  static constexpr int kRing = kWarps * kStages * slot_bytes<T, HD>();
+  static constexpr int kMinCtas = WIDE ? 1 : 3;
+  static_assert(kStages >= 2, "a unit in flight beside the one at work");
+};
 
 // ---------------------------------------------------------------------------
 // One warp's state over its units: FP16 cache.
 // ---------------------------------------------------------------------------
-template <int HD, int GP>
+template <int HD>
 struct WarpF16 {
   static constexpr int kUnit = 16;
   static constexpr int kPitch = HD * 2 + 16;
@@ -172,12 +240,12 @@ struct WarpF16 {
   float factor;             // score = product * factor (log2 units)
 
   // q of the group's heads, scaled and split into shared memory, then to registers.
+  template <int W>
   __device__ __forceinline__ void init(const float* q, int G, float scale_log2, char* scratch,
-                                       int warp, int lane) {
+                                       uint4*, int warp, int lane) {
     __half* s_q = reinterpret_cast<__half*>(scratch);                 // [16][HD + 8]
     float* s_f = reinterpret_cast<float*>(scratch + 16 * kPitch);     // [8]
-    {
-      const int h = warp;  // one head a warp
+    for (int h = warp; h < 8; h += W) {  // one head a warp at a time
       float x[HD / 32], big = 0.f;
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {
@@ -212,31 +280,39 @@ struct WarpF16 {
   }
 
   template <bool WEIGHTS>
-  __device__ __forceinline__ void step(uint32_t slot, int rows, float* scores, int G, float*,
-                                       int lane) {
+  __device__ __forceinline__ void step(uint32_t slot, int rows, float* scores, int64_t pitch,
+                                       int G, const uint4*, int lane) {
     float s[2][2];
     const int sub = lane >> 3, in = lane & 7;
 #pragma unroll
     for (int nt = 0; nt < 2; ++nt) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      // accumulators of 32 channels each, added in FP32: the matrix instruction
+      // truncates, and a chain over all channels did so on the whole sum
+      // (1.5e-6 of the output over 131,072 rows; 0.7e-6 this way), and waited longer
+      float c[HD / 32][4];
       const uint32_t base = slot + (nt * 8 + in) * kPitch + sub * 16;
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ks += 2) {
+      for (int j = 0; j < HD / 32; ++j) {
+        c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
         uint32_t b[4];
-        ldmatrix_x4(b, base + ks * 32);
-        mma_f16(c, qa[ks], b[0], b[1]);
-        mma_f16(c, qa[ks + 1], b[2], b[3]);
+        ldmatrix_x4(b, base + j * 64);
+        mma_f16(c[j], qa[2 * j], b[0], b[1]);
+        mma_f16(c[j], qa[2 * j + 1], b[2], b[3]);
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int r = nt * 8 + 2 * (lane & 3) + j;
-        s[nt][j] = (c[j] + c[2 + j]) * factor;
-        if (r >= rows) {
-          s[nt][j] = -INFINITY;
-        } else if (WEIGHTS && (lane >> 2) < G) {
-          __stcg(scores + (int64_t)r * G + (lane >> 2), s[nt][j]);
+        float hi = c[0][j], lo = c[0][2 + j];
+#pragma unroll
+        for (int i = 1; i < HD / 32; ++i) {
+          hi += c[i][j];
+          lo += c[i][2 + j];
         }
+        s[nt][j] = r < rows ? (hi + lo) * factor : -INFINITY;
       }
+      if (WEIGHTS && (lane >> 2) < G)  // the pitch has room for a whole unit
+        __stcg(reinterpret_cast<float2*>(scores + (lane >> 2) * pitch + nt * 8 + 2 * (lane & 3)),
+               make_float2(s[nt][0], s[nt][1]));
     }
     float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -279,7 +355,6 @@ struct WarpF16 {
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     const int h = lane >> 2;
-    if (h >= GP) return;
     if ((lane & 3) == 0) {
       ml[h * 2] = m;
       ml[h * 2 + 1] = l;
@@ -293,220 +368,192 @@ struct WarpF16 {
   }
 };
 
-// Sums N = 4 * GP values over the 16 lanes of a half-warp by halving exchanges;
-// lane l then holds the values of row (l >> 2) & 3 and heads starting at
-// (l & 3) * GP / 4 (GP < 4: head (l & 3) * GP >> 2), GP / 4 (at least one) of them.
-template <int N>
-__device__ __forceinline__ void half_warp_scatter(float (&v)[N], int lane) {
-  int n = N;
-#pragma unroll
-  for (int m = 8; m > 0; m >>= 1) {
-    if (n > 1) {
-      n >>= 1;
-      const bool up = (lane & m) != 0;
-#pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        if (i < n) {
-          const float keep = up ? v[i + n] : v[i];
-          const float send = up ? v[i] : v[i + n];
-          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, m);
-        }
-      }
-    } else {
-      v[0] += __shfl_xor_sync(0xffffffffu, v[0], m);
-    }
-  }
-}
-
 // ---------------------------------------------------------------------------
-// FP32 cache.  Scores: lane = (row group lane / 16, part lane % 16); a part
-// holds HD / 16 channels of all heads of q in registers, a row group the rows
-// rg, rg + 2, rg + 4, rg + 6 of a unit.  Outputs: a lane owns HD / 32 channels
-// of every head.
+// FP32 cache.  The fragments of q, both halves, lie in shared memory in the order
+// the lanes read them.  A product's row order within a unit is free: C of the
+// scores leaves a lane rows 2 (lane & 3) and + 1, which are k indices lane & 3 and
+// + 4 of the second product, so p needs no exchange; and a lane's two output
+// columns of a pair of tiles are neighbours, read by one 8-byte load.  With
+// pitches of HD + 4 floats all these loads are free of bank conflicts.
 // ---------------------------------------------------------------------------
-template <int HD, int GP>
+template <int HD>
 struct WarpF32 {
   static constexpr int kUnit = 8;
   static constexpr int kPitch = HD * 4 + 16;
-  static constexpr int kPairs = HD / 32;       // channel pairs of a part
-  static constexpr int kHpl = GP >= 4 ? GP / 4 : 1;
-  static constexpr int kOwn = HD / 32;         // output channels of a lane
-  uint64_t qr[GP][kPairs];
-  float o[GP][kOwn];
-  float m[kHpl], l[kHpl];
+  float o[HD / 8][4];  // tile pair j: columns 16 j + 2 n (tile 2 j) and + 1 (tile 2 j + 1)
+  float m, l;          // head lane / 4; l: this lane's share of the sum
   float factor;
 
-  // Channel of pair j of a part: part-major 8-byte chunks, 16 parts side by side.
-  __device__ __forceinline__ void init(const float* q, int G, float scale_log2, char*, int,
-                                       int lane) {
-    const int part = lane & 15;
-#pragma unroll
-    for (int h = 0; h < GP; ++h) {
-#pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        float2 x = make_float2(0.f, 0.f);
-        if (h < G) x = *reinterpret_cast<const float2*>(q + (int64_t)h * HD + (j * 16 + part) * 2);
-        qr[h][j] = pk2(x.x, x.y);
+  template <int W>
+  __device__ __forceinline__ void init(const float* q, int G, float scale_log2, char*, uint4* s_q,
+                                       int warp, int lane) {
+    // fragment of step ks: (hi, lo) of channels 8 ks + (lane & 3) and + 4 of head lane / 4
+    for (int i = warp * 32 + lane; i < HD / 8 * 32; i += W * 32) {
+      const int l = i & 31, h = l >> 2, ch = (i >> 5) * 8 + (l & 3);
+      float x = 0.f, y = 0.f;
+      if (h < G) {
+        x = q[(int64_t)h * HD + ch];
+        y = q[(int64_t)h * HD + ch + 4];
       }
-#pragma unroll
-      for (int j = 0; j < kOwn; ++j) o[h][j] = 0.f;
+      uint4 f;
+      split_tf32(x, f.x, f.y);
+      split_tf32(y, f.z, f.w);
+      s_q[i] = f;
     }
+    __syncthreads();
     factor = scale_log2;
 #pragma unroll
-    for (int j = 0; j < kHpl; ++j) {
-      m[j] = -INFINITY;
-      l[j] = 0.f;
-    }
+    for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
   }
 
   template <bool WEIGHTS>
-  __device__ __forceinline__ void step(uint32_t slot, int rows, float* scores, int G, float* sp,
-                                       int lane) {
-    const int part = lane & 15, rg = lane >> 4;
-    float acc[4 * GP];
+  __device__ __forceinline__ void step(uint32_t slot, int rows, float* scores, int64_t pitch,
+                                       int G, const uint4* s_q, int lane) {
+    // scores: accumulators of 32 channels each, added in FP32 (see WarpF16)
+    float c[HD / 32][4];
+    const uint32_t kbase = slot + (lane >> 2) * kPitch + (lane & 3) * 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t base = slot + (rg + 2 * i) * kPitch + part * 8;
-      uint64_t kx[kPairs];
+    for (int j = 0; j < HD / 32; ++j) {
+      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j)
-        asm volatile("ld.shared.b64 %0, [%1];" : "=l"(kx[j]) : "r"(base + j * 128));
-#pragma unroll
-      for (int h = 0; h < GP; ++h) {
-        uint64_t a = mul2(qr[h][0], kx[0]);
-#pragma unroll
-        for (int j = 1; j < kPairs; ++j) a = fma2(qr[h][j], kx[j], a);
-        float x, y;
-        upk2(a, x, y);
-        acc[i * GP + h] = x + y;
+      for (int i = 0; i < 4; ++i) {
+        const int ks = 4 * j + i;
+        const uint4 a = s_q[ks * 32 + lane];
+        uint32_t h0, l0, h1, l1;
+        split_tf32(lds_f32(kbase + ks * 32), h0, l0);
+        split_tf32(lds_f32(kbase + ks * 32 + 16), h1, l1);
+        mma_tf32(c[j], a, h0, h1);
+        mma_tf32(c[j], a, l0, l1);
       }
     }
-    half_warp_scatter<4 * GP>(acc, lane);
-    const int r = rg + 2 * ((lane >> 2) & 3);
-    const int h0 = ((lane & 3) * GP) >> 2;
-    // GP < 4: lanes that share a (row, head) hold the same sum; one of them counts
-    const bool first = GP >= 4 || (((lane & 3) * GP) & 3) == 0;
-    float a[kHpl];
-    bool moved = false;
+    float s[2];
 #pragma unroll
-    for (int j = 0; j < kHpl; ++j) {
-      float s = acc[j] * factor;
-      if (r >= rows) {
-        s = -INFINITY;
-      } else if (WEIGHTS && first && h0 + j < G) {
-        __stcg(scores + (int64_t)r * G + h0 + j, s);
+    for (int j = 0; j < 2; ++j) {
+      float hi = c[0][j], lo = c[0][2 + j];
+#pragma unroll
+      for (int i = 1; i < HD / 32; ++i) {
+        hi += c[i][j];
+        lo += c[i][2 + j];
       }
-      float top = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, 4));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-      const float m_new = fmaxf(m[j], top);
-      const float ref = m_new == -INFINITY ? 0.f : m_new;
-      a[j] = m[j] == m_new ? 1.f : exp2_approx(m[j] - ref);
-      moved |= m[j] != m_new;
-      m[j] = m_new;
-      const float pr = exp2_approx(s - ref);
-      l[j] = l[j] * a[j] + (first ? pr : 0.f);
-      // sp: p [8 rows][GP], then the factors of the old output [GP]
-      if (first) sp[r * GP + h0 + j] = pr;
-      if (first && r == 0) sp[8 * GP + h0 + j] = a[j];
+      s[j] = 2 * (lane & 3) + j < rows ? (hi + lo) * factor : -INFINITY;
     }
-    const bool any = __any_sync(0xffffffffu, moved);
-    __syncwarp();
-    if (any) {
+    if (WEIGHTS && (lane >> 2) < G)
+      __stcg(reinterpret_cast<float2*>(scores + (lane >> 2) * pitch + 2 * (lane & 3)),
+             make_float2(s[0], s[1]));
+    float top = fmaxf(s[0], s[1]);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float m_new = fmaxf(m, top);
+    const float ref = m_new == -INFINITY ? 0.f : m_new;
+    if (__any_sync(0xffffffffu, m_new != m)) {
+      const float a = m == m_new ? 1.f : exp2_approx(m - ref);
+      l *= a;
 #pragma unroll
-      for (int h = 0; h < GP; ++h) {
-        const float x = sp[8 * GP + h];
+      for (int i = 0; i < HD / 8; ++i)
 #pragma unroll
-        for (int j = 0; j < kOwn; ++j) o[h][j] *= x;
-      }
+        for (int j = 0; j < 4; ++j) o[i][j] *= a;
+      m = m_new;
     }
-    const uint32_t vbase = slot + kUnit * kPitch;
+    const float p0 = exp2_approx(s[0] - ref), p1 = exp2_approx(s[1] - ref);
+    l += p0 + p1;
+    uint4 pa;  // k index lane & 3: row 2 (lane & 3); + 4: the row after it
+    split_tf32(p0, pa.x, pa.y);
+    split_tf32(p1, pa.z, pa.w);
+    const uint32_t vbase = slot + kUnit * kPitch + 2 * (lane & 3) * kPitch + (lane >> 2) * 8;
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      float v[kOwn];
-      const uint32_t at = vbase + t * kPitch;
-      if constexpr (kOwn == 4) {
-        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
-                     : "r"(at + lane * 16));
-      } else if constexpr (kOwn == 2) {
-        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(at + lane * 8));
-      } else {
+    for (int j = 0; j < HD / 16; ++j) {
+      float v0[2], v1[2];  // this lane's two columns of its two rows
+      lds_f32x2(vbase + j * 64, v0);
+      lds_f32x2(vbase + kPitch + j * 64, v1);
 #pragma unroll
-        for (int j = 0; j < kOwn; ++j) v[j] = lds_f32(at + (j * 32 + lane) * 4);
-      }
-#pragma unroll
-      for (int h = 0; h < GP; ++h) {
-        const float pr = sp[t * GP + h];
-#pragma unroll
-        for (int j = 0; j < kOwn; ++j) o[h][j] = fmaf(pr, v[j], o[h][j]);
+      for (int i = 0; i < 2; ++i) {
+        uint32_t h0, l0, h1, l1;
+        split_tf32(v0[i], h0, l0);
+        split_tf32(v1[i], h1, l1);
+        mma_tf32(o[2 * j + i], pa, h0, h1);
+        mma_tf32(o[2 * j + i], pa, l0, l1);
       }
     }
-    __syncwarp();
   }
 
   __device__ __forceinline__ void store(float* so, float* ml, int lane) {
-    const int h0 = ((lane & 3) * GP) >> 2;
-#pragma unroll
-    for (int j = 0; j < kHpl; ++j) {
-      float x = l[j];
-      x += __shfl_xor_sync(0xffffffffu, x, 4);
-      x += __shfl_xor_sync(0xffffffffu, x, 8);
-      x += __shfl_xor_sync(0xffffffffu, x, 16);
-      if (GP == 1) {
-        // lanes 0-3 hold the one head; only lane 0 of each quad counted
-        x = __shfl_sync(0xffffffffu, x, 0);
-      } else if (GP == 2) {
-        x = __shfl_sync(0xffffffffu, x, lane & ~1);
-      }
-      if (lane < 4) {
-        ml[(h0 + j) * 2] = m[j];
-        ml[(h0 + j) * 2 + 1] = x;
-      }
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const int h = lane >> 2;
+    if ((lane & 3) == 0) {
+      ml[h * 2] = m;
+      ml[h * 2 + 1] = l;
     }
+    // C of a tile: columns n = 2 (lane & 3) and + 1 of head h
 #pragma unroll
-    for (int h = 0; h < GP; ++h)
+    for (int j = 0; j < HD / 16; ++j)
 #pragma unroll
-      for (int j = 0; j < kOwn; ++j)
-        so[h * HD + (kOwn == 3 ? j * 32 + lane : lane * kOwn + j)] = o[h][j];
+      for (int e = 0; e < 2; ++e) {
+        const int n = 2 * (lane & 3) + e;
+        *reinterpret_cast<float2*>(so + h * HD + 16 * j + 2 * n) =
+            make_float2(o[2 * j][e] + o[2 * j][2 + e], o[2 * j + 1][e] + o[2 * j + 1][2 + e]);
+      }
   }
 };
 
-template <class T, int HD, int GP>
+template <class T, int HD>
 struct WarpOf;
-template <int HD, int GP>
-struct WarpOf<__half, HD, GP> {
-  using type = WarpF16<HD, GP>;
+template <int HD>
+struct WarpOf<__half, HD> {
+  using type = WarpF16<HD>;
 };
-template <int HD, int GP>
-struct WarpOf<float, HD, GP> {
-  using type = WarpF32<HD, GP>;
+template <int HD>
+struct WarpOf<float, HD> {
+  using type = WarpF32<HD>;
 };
 
+constexpr int GP = 8;  // heads of a product's row halves
+
+// The weight of a row, all heads of the group: sc its scores, norm (m, 1 / l) of each head.
+__device__ __forceinline__ float row_weight(const float* sc, int64_t pitch, const float* norm,
+                                            int G) {
+  float s[GP], x = 0.f;
+#pragma unroll
+  for (int h = 0; h < GP; ++h) s[h] = h < G ? __ldcg(sc + h * pitch) : 0.f;
+#pragma unroll
+  for (int h = 0; h < GP; ++h)
+    if (h < G) x = fmaf(exp2_approx(s[h] - norm[h * 2]), norm[h * 2 + 1], x);
+  return x;
+}
+
 // Shared memory: the warps' rings; after the stream the same bytes hold the
-// warps' outputs [kWarps][GP][HD], then (m, l) [kWarps][GP][2].  Static: the
-// CTA's joined output and (m, l), read by the other CTAs of the cluster.
-template <class T, int HD, int GP, bool BLOCKS, bool WEIGHTS>
-__global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_constant__ AttendParams p) {
-  using Warp = typename WarpOf<T, HD, GP>::type;
+// warps' outputs [kWarps][GP][HD] and (m, l) [kWarps][GP][2], then the CTA's joined
+// output [GP][HD], which the other CTAs of the cluster read as they do s_ml.
+template <class T, int HD, bool BLOCKS, bool WIDE>
+__global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::kMinCtas)
+    attend_kernel(const __grid_constant__ AttendParams p) {
+  using Warp = typename WarpOf<T, HD>::type;
+  using C = Cta<T, HD, WIDE>;
+  constexpr bool WEIGHTS = !BLOCKS;
+  constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kStages = C::kStages;
   constexpr int U = Warp::kUnit;
   constexpr int kShift = U == 16 ? 4 : 3;
-  constexpr int kStages = ring_stages<T, HD>();
   constexpr int kSlot = slot_bytes<T, HD>();
   extern __shared__ __align__(16) char s_ring[];
-  __shared__ __align__(16) float s_o[GP * HD];
   __shared__ float s_ml[GP * 2];
-  __shared__ float s_p[sizeof(T) == 4 ? kWarps * 9 * GP : 1];
+  __shared__ uint4 s_q[sizeof(T) == 4 ? HD / 8 * 32 : 1];  // FP32: q's fragments
   __shared__ float s_norm[GP * 2];
-  pdl_wait();
-  pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int S = p.S;
   const int rank = S > 1 ? (int)(blockIdx.x % (unsigned)S) : 0;
   const int item = (int)(blockIdx.x / (unsigned)S);
   const int b = item / p.n_kv, g = item - b * p.n_kv;
   const int G = p.n_heads / p.n_kv;
+  pdl_wait();
+  // Not when a join follows: its CTAs would take the first free places of this
+  // kernel's SMs and crowd there (109 us against 73 for 131,072 rows).
+  if (!p.part) pdl_launch_dependents();
   int32_t n = clamped_rows(p.n_pos, b, p.max_n_pos, p.status);
+  if (WEIGHTS && p.part && (int64_t)rank * p.part_rows >= n) return;
   const T* k = static_cast<const T*>(p.k_ptrs[b]);
   const T* v = static_cast<const T*>(p.v_ptrs[b]);
   if (!usable_ptrs(k, v, p.status)) n = 0;
@@ -515,14 +562,23 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
   k += (int64_t)g * HD;
   v += (int64_t)g * HD;
   const int32_t* ids = BLOCKS ? p.block_ids + (int64_t)item * p.n_sel : nullptr;
-  const int32_t units = BLOCKS ? (n > 0 ? p.n_sel << (p.br_shift - kShift) : 0)
-                               : (int32_t)(((int64_t)n + U - 1) / U);
-  const int32_t first = rank * kWarps + warp, stride = S * kWarps;
-  float* scores = WEIGHTS ? p.scores + (int64_t)item * p.max_n_pos * G : nullptr;
+  // units of this CTA's warps: a cluster's deal, or this part's
+  int32_t units = BLOCKS ? (n > 0 ? p.n_sel << (p.br_shift - kShift) : 0)
+                         : (int32_t)(((int64_t)n + U - 1) / U);
+  int32_t cta_first = rank * kWarps, stride = S * kWarps;
+  if (WEIGHTS && p.part) {
+    cta_first = rank * (p.part_rows / U);
+    units = min(units, cta_first + p.part_rows / U);
+    stride = kWarps;
+  }
+  const int32_t first = cta_first + warp;
+  float* scores = WEIGHTS ? p.scores + (int64_t)item * G * p.score_pitch : nullptr;
 
   const uint32_t ring = smem_u32(s_ring) + warp * (kStages * kSlot);
   Warp w;
-  w.init(p.q + ((int64_t)b * p.n_heads + (int64_t)g * G) * HD, G, p.scale_log2, s_ring, warp, lane);
+  w.template init<kWarps>(p.q + ((int64_t)b * p.n_heads + (int64_t)g * G) * HD, G, p.scale_log2,
+                          s_ring, s_q, warp, lane);
+  const uint64_t policy = WEIGHTS ? l2_evict_first_policy() : 0;
 
   // unit i of this warp is first + i * stride; its ring slot i % kStages
   const int32_t mine = units > first ? (units - first - 1) / stride + 1 : 0;
@@ -532,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
     row_of[i] = -1;
     if (i < mine) {
       row_of[i] = unit_row<BLOCKS, kShift>(p, ids, first + i * stride, n);
-      if (row_of[i] >= 0) load_unit<T, HD, U>(ring + i * kSlot, k, v, p.kv_stride, row_of[i], n, lane);
+      if (row_of[i] >= 0) load_unit<T, HD, U, WEIGHTS>(ring + i * kSlot, k, v, p.kv_bytes, row_of[i], n, policy, lane);
     }
     cp_async_commit();
   }
@@ -549,13 +605,14 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
         if (i + kAhead < mine) {
           row_of[ahead] = unit_row<BLOCKS, kShift>(p, ids, first + (i + kAhead) * stride, n);
           if (row_of[ahead] >= 0)
-            load_unit<T, HD, U>(ring + ahead * kSlot, k, v, p.kv_stride, row_of[ahead], n, lane);
+            load_unit<T, HD, U, WEIGHTS>(ring + ahead * kSlot, k, v, p.kv_bytes, row_of[ahead], n, policy,
+                                         lane);
         }
         cp_async_commit();
         const int32_t row0 = row_of[s];
         if (row0 >= 0)
-          w.template step<WEIGHTS>(ring + s * kSlot, n - row0, scores + (int64_t)row0 * G, G,
-                                   s_p + warp * 9 * GP, lane);
+          w.template step<WEIGHTS>(ring + s * kSlot, n - row0, scores + row0, p.score_pitch, G,
+                                   s_q, lane);
       }
     }
   }
@@ -565,8 +622,10 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
   // warps -> CTA
   float* so = reinterpret_cast<float*>(s_ring);
   float* sml = so + kWarps * GP * HD;
+  float* s_o = sml + kWarps * GP * 2;
   w.store(so + warp * GP * HD, sml + warp * GP * 2, lane);
   __syncthreads();
+  float* part = p.part + ((int64_t)item * S + rank) * G * (HD + 2);
   for (int i = tid; i < GP * HD; i += kThreads) {
     const int h = i / HD;
     float top = -INFINITY;
@@ -580,12 +639,23 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
       acc = fmaf(so[x * GP * HD + i], e, acc);
       sum = fmaf(sml[(x * GP + h) * 2 + 1], e, sum);
     }
+    if (WEIGHTS && p.part) {  // joined by attend_join_kernel
+      if (h < G) {
+        part[i] = acc;
+        if (i == h * HD) {
+          part[G * HD + h * 2] = top;
+          part[G * HD + h * 2 + 1] = sum;
+        }
+      }
+      continue;
+    }
     s_o[i] = acc;
     if (i == h * HD) {
       s_ml[h * 2] = top;
       s_ml[h * 2 + 1] = sum;
     }
   }
+  if (WEIGHTS && p.part) return;
   cluster_barrier(S);
 
   // CTAs -> result: each rank joins its share of the G x HD outputs
@@ -593,9 +663,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
   for (int i = rank * kThreads + tid; i < G * HD; i += S * kThreads) {
     const int h = i / HD;
     float top = -INFINITY;
+#pragma unroll 4
     for (int x = 0; x < S; ++x) top = fmaxf(top, S == 1 ? s_ml[h * 2] : *cluster_peer(&s_ml[h * 2], x));
     const float ref = top == -INFINITY ? 0.f : top;
     float acc = 0.f, sum = 0.f;
+#pragma unroll 4
     for (int x = 0; x < S; ++x) {
       const float* ml = S == 1 ? &s_ml[h * 2] : cluster_peer(&s_ml[h * 2], x);
       const float* ox = S == 1 ? &s_o[i] : cluster_peer(&s_o[i], x);
@@ -609,9 +681,11 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
   if constexpr (WEIGHTS) {
     if (tid < GP) {
       float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
       for (int x = 0; x < S; ++x)
         top = fmaxf(top, S == 1 ? s_ml[tid * 2] : *cluster_peer(&s_ml[tid * 2], x));
       const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
       for (int x = 0; x < S; ++x) {
         const float* ml = S == 1 ? &s_ml[tid * 2] : cluster_peer(&s_ml[tid * 2], x);
         sum = fmaf(ml[1], exp2_approx(ml[0] - ref), sum);
@@ -624,30 +698,118 @@ __global__ void __launch_bounds__(kThreads, 1) attend_kernel(const __grid_consta
   if constexpr (WEIGHTS) {
     // this CTA's own rows, in the order their units were dealt
     float* wrow = wts + (int64_t)g * p.weight_stride;
-    const int32_t cta_units = units > rank * kWarps ? (units - rank * kWarps - 1) / stride + 1 : 0;
+    const int32_t cta_units = units > cta_first ? (units - cta_first - 1) / stride + 1 : 0;
     const int64_t all = (int64_t)cta_units * kWarps * U;
     for (int64_t i = tid; i < all; i += kThreads) {
       const int32_t round = (int32_t)(i / (kWarps * U)), in = (int32_t)(i - (int64_t)round * kWarps * U);
-      const int64_t row = ((int64_t)rank * kWarps + (int64_t)round * stride) * U + in;
-      if (row >= n) continue;
-      const float* sc = scores + row * G;
-      float x = 0.f;
-      for (int h = 0; h < G; ++h)
-        x = fmaf(exp2_approx(__ldcg(sc + h) - s_norm[h * 2]), s_norm[h * 2 + 1], x);
-      wrow[row] += x;
+      const int64_t row = ((int64_t)cta_first + (int64_t)round * stride) * U + in;
+      if (row < n) wrow[row] += row_weight(scores + row, p.score_pitch, s_norm, G);
     }
   }
 }
 
-template <class T, int HD, int GP, bool BLOCKS>
+// Joins the S parts of every item, normalises, and adds the weights: each CTA
+// takes a share of an item's outputs and kJoinRows of its rows.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinRows = 1024;
+
+__global__ void __launch_bounds__(kJoinThreads)
+    attend_join_kernel(const __grid_constant__ AttendParams p, int32_t head_dim, int32_t shares) {
+  __shared__ float s_norm[GP * 2];
+  __shared__ float s_acc[kJoinThreads / 32][32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int item = (int)(blockIdx.x / (unsigned)shares), share = (int)(blockIdx.x % (unsigned)shares);
+  const int b = item / p.n_kv, g = item - b * p.n_kv;
+  const int G = p.n_heads / p.n_kv;
+  pdl_wait();
+  pdl_launch_dependents();
+  int32_t n = clamped_rows(p.n_pos, b, p.max_n_pos, p.status);
+  float* wts = p.weight_ptrs[b];
+  if (!usable_weights(wts, p.status)) n = 0;
+  if (!usable_ptrs(p.k_ptrs[b], p.v_ptrs[b], p.status)) n = 0;
+  const int32_t S = (int32_t)(((int64_t)n + p.part_rows - 1) / p.part_rows);  // parts with rows
+  const int64_t row0 = (int64_t)share * kJoinRows, row1 = min(row0 + kJoinRows, (int64_t)n);
+  if (row0 >= row1 && share * 32 >= G * head_dim) return;
+  const int64_t len = (int64_t)G * (head_dim + 2);
+  const float* part = p.part + (int64_t)item * p.S * len;
+  // one head a warp: its largest m and its sum
+  if (warp < G) {
+    const float* ml = part + (int64_t)G * head_dim + warp * 2;
+    float top = -INFINITY;
+    for (int x = lane; x < S; x += 32) top = fmaxf(top, ml[x * len]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f;
+    for (int x = lane; x < S; x += 32) sum = fmaf(ml[x * len + 1], exp2_approx(ml[x * len] - ref), sum);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) {
+      s_norm[warp * 2] = ref;
+      s_norm[warp * 2 + 1] = sum == 0.f ? 0.f : 1.0f / sum;  // no rows: zeros
+    }
+  }
+  __syncthreads();
+  const float* scores = p.scores + (int64_t)item * G * p.score_pitch;
+  float* wrow = wts + (int64_t)g * p.weight_stride;
+#pragma unroll 2
+  for (int64_t row = row0 + tid; row < row1; row += kJoinThreads)
+    wrow[row] += row_weight(scores + row, p.score_pitch, s_norm, G);
+  // outputs: 32 at a time, a warp for every eighth part
+  float* out = p.xb + ((int64_t)b * p.n_heads + (int64_t)g * G) * head_dim;
+  for (int i0 = share * 32; i0 < G * head_dim; i0 += shares * 32) {
+    const int i = i0 + lane, h = i / head_dim;  // G * head_dim is a multiple of 32
+    float acc = 0.f;
+#pragma unroll 4
+    for (int x = warp; x < S; x += kJoinThreads / 32)
+      acc = fmaf(part[x * len + i], exp2_approx(part[x * len + G * head_dim + h * 2] - s_norm[h * 2]), acc);
+    s_acc[warp][lane] = acc;
+    __syncthreads();
+    if (warp == 0) {
+      acc = 0.f;
+#pragma unroll
+      for (int x = 0; x < kJoinThreads / 32; ++x) acc += s_acc[x][lane];
+      out[i] = acc * s_norm[h * 2 + 1];
+    }
+    __syncthreads();
+  }
+}
+
+// Rows of a part when a second kernel joins the parts, 0 when a cluster does.
+// Parts are sized for two waves of CTAs (three an SM) over a batch whose
+// sequences are all as long as the longest, and take at least 8 units a warp;
+// sequences too short for two such parts are left to a cluster (one launch
+// less, about 3 us).
+int32_t part_rows_for(int64_t items, int64_t max_rows, int unit, const DeviceInfo& dev) {
+  const int64_t step = 4 * unit, least = 8 * step;
+  int64_t rows = (max_rows * items + 6 * dev.sms - 1) / (6 * dev.sms);
+  rows = std::max(least, (rows + step - 1) / step * step);
+  return max_rows > rows ? (int32_t)rows : 0;
+}
+
+// Floats between the heads' scores: a last unit stores its rows past the end too.
+int64_t score_pitch_for(int64_t max_rows) { return (max_rows + 15) / 16 * 16; }
+
+template <class T, int HD, bool BLOCKS, bool WIDE>
+int launch_shape(AttendParams& p, int64_t items, int S, cudaStream_t stream, std::string* err) {
+  static std::atomic<uint64_t> attr_done{0};
+  using C = Cta<T, HD, WIDE>;
+  static_assert(C::kRing >= (C::kWarps * (HD + 2) + HD) * GP * 4, "the outputs reuse the rings");
+  static_assert(C::kRing >= 16 * (HD * 2 + 16) + 32, "q is split in the rings");
+  if (items * S > INT32_MAX) {
+    *err = "batch * n_kv_heads too large";
+    return GLA_ERR_NOT_SUPPORTED;
+  }
+  p.S = S;
+  return launch_clusters(attend_kernel<T, HD, BLOCKS, WIDE>, (unsigned)(items * S),
+                         C::kThreads, (size_t)C::kRing, p.part ? 1 : S, attr_done, stream,
+                         "attention", err, p);
+}
+
+template <class T, int HD, bool BLOCKS>
 int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,
                std::string* err) {
-  static std::atomic<uint64_t> attr_done{0};
-  constexpr bool WEIGHTS = !BLOCKS;
   constexpr int U = unit_rows<T, HD>();
-  constexpr size_t ring = (size_t)kWarps * ring_stages<T, HD>() * slot_bytes<T, HD>();
-  static_assert(ring >= (size_t)kWarps * GP * (HD + 2) * 4, "the outputs reuse the rings");
-  static_assert(ring >= 16 * (HD * 2 + 16) + 32, "q is split in the rings");
   AttendParams p{};
   p.q = r.q;
   p.k_ptrs = r.k_ptrs;
@@ -657,7 +819,7 @@ int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t strea
   p.xb = r.xb;
   p.n_heads = r.n_heads;
   p.n_kv = r.n_kv;
-  p.kv_stride = r.kv_stride;
+  p.kv_bytes = (uint32_t)(r.kv_stride * (int64_t)sizeof(T));
   p.scale_log2 = r.scale * kLog2e;
   p.block_ids = r.block_ids;
   p.n_sel = r.n_sel;
@@ -666,53 +828,64 @@ int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t strea
   p.weight_stride = r.weight_stride;
   p.scores = r.scores;
   p.status = r.status;
-  const int64_t rows = BLOCKS ? std::min<int64_t>((int64_t)r.n_sel * r.block_rows, INT32_MAX)
-                              : (int64_t)r.max_n_pos;
+  const int64_t rows = BLOCKS ? (int64_t)r.n_sel * r.block_rows : (int64_t)r.max_n_pos;
   const int64_t units = (rows + U - 1) / U;
   const int64_t items = (int64_t)r.batch * r.n_kv;
-  // CTAs a (sequence, kv head): as many as fill the device once, while every
-  // warp still has a unit
-  int S = 1;
-  while (S < 16 && items * S < dev.sms && units > (int64_t)kWarps * S) S *= 2;
-  p.S = S;
-  if (items * S > INT32_MAX) {
-    *err = "batch * n_kv_heads too large";
-    return GLA_ERR_NOT_SUPPORTED;
+  if constexpr (!BLOCKS) {
+    p.score_pitch = score_pitch_for(r.max_n_pos);
+    p.part_rows = part_rows_for(items, r.max_n_pos, U, dev);
+    if (p.part_rows) {
+      const int64_t parts = ((int64_t)r.max_n_pos + p.part_rows - 1) / p.part_rows;
+      const int64_t shares = ((int64_t)r.max_n_pos + kJoinRows - 1) / kJoinRows;
+      if (items * parts > INT32_MAX || items * shares > INT32_MAX) {
+        *err = "batch * n_kv_heads * max_n_pos too large";
+        return GLA_ERR_NOT_SUPPORTED;
+      }
+      p.part = r.scores + (size_t)(items * (r.n_heads / r.n_kv)) * p.score_pitch;
+      int rc = launch_shape<T, HD, BLOCKS, false>(p, items, (int)parts, stream, err);
+      if (rc != GLA_OK) return rc;
+      static std::atomic<uint64_t> attr_done{0};
+      return launch_clusters(attend_join_kernel, (unsigned)(items * shares), kJoinThreads, 0, 1,
+                             attr_done, stream, "attention join", err, p, (int32_t)HD,
+                             (int32_t)shares);
+    }
   }
-  return launch_clusters(attend_kernel<T, HD, GP, BLOCKS, WEIGHTS>, (unsigned)(items * S), kThreads,
-                         ring, S, attr_done, stream, "attention", err, p);
-}
-
-template <class T, int HD, int GP>
-int by_mode(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream, std::string* err) {
-  return r.block_ids ? launch_one<T, HD, GP, true>(r, dev, stream, err)
-                     : launch_one<T, HD, GP, false>(r, dev, stream, err);
+  // CTAs of a cluster: as many as fill the device, while every warp still has a
+  // unit; wide ones if 16 slim ones an item would not fill it
+  const bool wide = items * 16 < 3 * dev.sms;
+  const int warps = wide ? 8 : 4;
+  const int64_t slots = wide ? dev.sms : 3 * dev.sms;
+  int S = 1;
+  while (S < 16 && items * S < slots && units > (int64_t)warps * S) S *= 2;
+  return wide ? launch_shape<T, HD, BLOCKS, true>(p, items, S, stream, err)
+              : launch_shape<T, HD, BLOCKS, false>(p, items, S, stream, err);
 }
 
 template <int HD>
-int by_group(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,
-             std::string* err) {
-  // FP16: the matrix instruction takes 8 heads whatever the group
-  if (r.dtype == GLA_DTYPE_F16) return by_mode<__half, HD, 8>(r, dev, stream, err);
-  const int G = r.n_heads / r.n_kv;
-  if (G == 1) return by_mode<float, HD, 1>(r, dev, stream, err);
-  if (G == 2) return by_mode<float, HD, 2>(r, dev, stream, err);
-  if (G <= 4) return by_mode<float, HD, 4>(r, dev, stream, err);
-  return by_mode<float, HD, 8>(r, dev, stream, err);
+int by_type(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream, std::string* err) {
+  if (r.dtype == GLA_DTYPE_F16)
+    return r.block_ids ? launch_one<__half, HD, true>(r, dev, stream, err)
+                       : launch_one<__half, HD, false>(r, dev, stream, err);
+  return r.block_ids ? launch_one<float, HD, true>(r, dev, stream, err)
+                     : launch_one<float, HD, false>(r, dev, stream, err);
 }
 
 }  // namespace
 
-size_t attend_score_floats(const AttendRequest& r) {
-  return (size_t)r.batch * r.n_heads * (size_t)r.max_n_pos;
+size_t attend_score_floats(const AttendRequest& r, const DeviceInfo& dev) {
+  const int unit = r.dtype == GLA_DTYPE_F16 ? unit_rows<__half, 64>() : unit_rows<float, 64>();
+  const int64_t rows = part_rows_for((int64_t)r.batch * r.n_kv, r.max_n_pos, unit, dev);
+  const int64_t parts = rows ? ((int64_t)r.max_n_pos + rows - 1) / rows : 0;
+  return (size_t)r.batch * r.n_heads *
+         (size_t)(score_pitch_for(r.max_n_pos) + parts * (r.head_dim + 2));
 }
 
 int launch_attend(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,
                   std::string* err) {
   switch (r.head_dim) {
-    case 64: return by_group<64>(r, dev, stream, err);
-    case 96: return by_group<96>(r, dev, stream, err);
-    default: return by_group<128>(r, dev, stream, err);
+    case 64: return by_type<64>(r, dev, stream, err);
+    case 96: return by_type<96>(r, dev, stream, err);
+    default: return by_type<128>(r, dev, stream, err);
   }
 }
 
