@@ -149,7 +149,8 @@ struct AttendParams {
   int64_t weight_stride;
   float* scores;      // [item][G][score_pitch]
   int64_t score_pitch;
-  float* part;        // [item][S][G][HD + 2]: o, then (m, l) of each head
+  float* part;        // o of the parts: [item][S][G][HD]
+  float2* part_ml;    // their (m, l): [item][G][S]
   int32_t part_rows;  // of a part
   int32_t* status;
 };
@@ -549,8 +550,9 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   const int b = item / p.n_kv, g = item - b * p.n_kv;
   const int G = p.n_heads / p.n_kv;
   pdl_wait();
-  // Not when a join follows: its CTAs would take the first free places of this
-  // kernel's SMs and crowd there (109 us against 73 for 131,072 rows).
+  // A join that follows is let in only behind the stream: its CTAs would take the
+  // first free places of this kernel's SMs and crowd there (109 us against 73 for
+  // 131,072 rows).
   if (!p.part) pdl_launch_dependents();
   int32_t n = clamped_rows(p.n_pos, b, p.max_n_pos, p.status);
   if (WEIGHTS && p.part && (int64_t)rank * p.part_rows >= n) return;
@@ -580,43 +582,38 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
                           s_ring, s_q, warp, lane);
   const uint64_t policy = WEIGHTS ? l2_evict_first_policy() : 0;
 
-  // unit i of this warp is first + i * stride; its ring slot i % kStages
+  // unit i of this warp is first + i * stride; its ring slot i % kStages.  A slot
+  // is filled again as soon as it is read out, so while a warp waits for a unit the
+  // ring's other units are under way too.
   const int32_t mine = units > first ? (units - first - 1) / stride + 1 : 0;
   int32_t row_of[kStages];
-#pragma unroll
-  for (int i = 0; i < kStages - 1; ++i) {
-    row_of[i] = -1;
+  auto fetch = [&](int s, int32_t i) {
+    row_of[s] = -1;
     if (i < mine) {
-      row_of[i] = unit_row<BLOCKS, kShift>(p, ids, first + i * stride, n);
-      if (row_of[i] >= 0) load_unit<T, HD, U, WEIGHTS>(ring + i * kSlot, k, v, p.kv_bytes, row_of[i], n, policy, lane);
+      row_of[s] = unit_row<BLOCKS, kShift>(p, ids, first + i * stride, n);
+      if (row_of[s] >= 0)
+        load_unit<T, HD, U, WEIGHTS>(ring + s * kSlot, k, v, p.kv_bytes, row_of[s], n, policy, lane);
     }
     cp_async_commit();
-  }
+  };
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) fetch(s, s);
   for (int32_t i0 = 0; i0 < mine; i0 += kStages) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) {
-      const int32_t i = i0 + s;
-      if (i < mine) {
-        constexpr int kAhead = kStages - 1;
-        const int ahead = (s + kAhead) % kStages;
-        cp_async_wait<kStages - 2>();
-        __syncwarp();  // unit i is here for every lane, and slot `ahead` is read out
-        row_of[ahead] = -1;
-        if (i + kAhead < mine) {
-          row_of[ahead] = unit_row<BLOCKS, kShift>(p, ids, first + (i + kAhead) * stride, n);
-          if (row_of[ahead] >= 0)
-            load_unit<T, HD, U, WEIGHTS>(ring + ahead * kSlot, k, v, p.kv_bytes, row_of[ahead], n, policy,
-                                         lane);
-        }
-        cp_async_commit();
-        const int32_t row0 = row_of[s];
-        if (row0 >= 0)
-          w.template step<WEIGHTS>(ring + s * kSlot, n - row0, scores + row0, p.score_pitch, G,
-                                   s_q, lane);
+      if (i0 + s < mine) {
+        cp_async_wait<kStages - 1>();
+        __syncwarp();  // the unit is here for every lane
+        if (row_of[s] >= 0)
+          w.template step<WEIGHTS>(ring + s * kSlot, n - row_of[s], scores + row_of[s],
+                                   p.score_pitch, G, s_q, lane);
+        __syncwarp();  // and read out by every lane
+        fetch(s, i0 + s + kStages);
       }
     }
   }
   cp_async_wait<0>();
+  if (p.part) pdl_launch_dependents();
   __syncthreads();  // rings drained
 
   // warps -> CTA
@@ -625,7 +622,7 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   float* s_o = sml + kWarps * GP * 2;
   w.store(so + warp * GP * HD, sml + warp * GP * 2, lane);
   __syncthreads();
-  float* part = p.part + ((int64_t)item * S + rank) * G * (HD + 2);
+  float* part = p.part + ((int64_t)item * S + rank) * G * HD;
   for (int i = tid; i < GP * HD; i += kThreads) {
     const int h = i / HD;
     float top = -INFINITY;
@@ -642,10 +639,7 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
     if (WEIGHTS && p.part) {  // joined by attend_join_kernel
       if (h < G) {
         part[i] = acc;
-        if (i == h * HD) {
-          part[G * HD + h * 2] = top;
-          part[G * HD + h * 2 + 1] = sum;
-        }
+        if (i == h * HD) p.part_ml[((int64_t)item * G + h) * S + rank] = make_float2(top, sum);
       }
       continue;
     }
@@ -708,81 +702,122 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   }
 }
 
-// Joins the S parts of every item, normalises, and adds the weights: each CTA
-// takes a share of an item's outputs and kJoinRows of its rows.
+// Joins the parts of every item.  Of an item's CTAs the first `out_shares` add up
+// 32 outputs each, the others normalise kJoinRows rows' scores and add the
+// weights.  Latency-bound: everything that does not need the joined (m, l) is
+// loaded before they are known.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinRows = 1024;
+constexpr int kJoinRows = 512;
 
 __global__ void __launch_bounds__(kJoinThreads)
-    attend_join_kernel(const __grid_constant__ AttendParams p, int32_t head_dim, int32_t shares) {
+    attend_join_kernel(const __grid_constant__ AttendParams p, int32_t head_dim,
+                       int32_t out_shares, int32_t shares) {
   __shared__ float s_norm[GP * 2];
   __shared__ float s_acc[kJoinThreads / 32][32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int item = (int)(blockIdx.x / (unsigned)shares), share = (int)(blockIdx.x % (unsigned)shares);
+  const int item = (int)(blockIdx.x / (unsigned)shares);
+  const int share = (int)(blockIdx.x % (unsigned)shares) - out_shares;
   const int b = item / p.n_kv, g = item - b * p.n_kv;
   const int G = p.n_heads / p.n_kv;
   pdl_wait();
   pdl_launch_dependents();
   int32_t n = clamped_rows(p.n_pos, b, p.max_n_pos, p.status);
   float* wts = p.weight_ptrs[b];
-  if (!usable_weights(wts, p.status)) n = 0;
-  if (!usable_ptrs(p.k_ptrs[b], p.v_ptrs[b], p.status)) n = 0;
+  if (!usable_weights(wts, p.status) || !usable_ptrs(p.k_ptrs[b], p.v_ptrs[b], p.status)) n = 0;
+  const int64_t row0 = (int64_t)share * kJoinRows;
+  if (share < 0 && n == 0) {  // no rows: zeros
+    if (tid < 32)
+      p.xb[((int64_t)b * p.n_heads + (int64_t)g * G) * head_dim + (share + out_shares) * 32 + tid] = 0.f;
+    return;
+  }
+  if (row0 >= n) return;
   const int32_t S = (int32_t)(((int64_t)n + p.part_rows - 1) / p.part_rows);  // parts with rows
-  const int64_t row0 = (int64_t)share * kJoinRows, row1 = min(row0 + kJoinRows, (int64_t)n);
-  if (row0 >= row1 && share * 32 >= G * head_dim) return;
-  const int64_t len = (int64_t)G * (head_dim + 2);
-  const float* part = p.part + (int64_t)item * p.S * len;
-  // one head a warp: its largest m and its sum
-  if (warp < G) {
-    const float* ml = part + (int64_t)G * head_dim + warp * 2;
+  const float2* ml = p.part_ml + (int64_t)item * G * p.S;
+
+  constexpr int kPer = kJoinRows / kJoinThreads;
+  float s[kPer][GP], old[kPer];
+  float* wrow = wts + (int64_t)g * p.weight_stride + row0;
+  const float* scores = p.scores + (int64_t)item * G * p.score_pitch + row0;
+  if (share >= 0) {
+#pragma unroll
+    for (int r = 0; r < kPer; ++r) {
+      const int i = r * kJoinThreads + tid;
+      if (row0 + i < n) {
+        old[r] = wrow[i];
+#pragma unroll
+        for (int h = 0; h < GP; ++h)
+          if (h < G) s[r][h] = __ldcg(scores + h * p.score_pitch + i);
+      }
+    }
+  }
+  // one head a warp (an output share needs only its own): its largest m and its sum
+  const int out0 = (share + out_shares) * 32, out_head = out0 / head_dim;
+  if (warp < G && (share >= 0 || warp == out_head)) {
     float top = -INFINITY;
-    for (int x = lane; x < S; x += 32) top = fmaxf(top, ml[x * len]);
+#pragma unroll 8
+    for (int x = lane; x < S; x += 32) top = fmaxf(top, ml[warp * p.S + x].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     const float ref = top == -INFINITY ? 0.f : top;
     float sum = 0.f;
-    for (int x = lane; x < S; x += 32) sum = fmaf(ml[x * len + 1], exp2_approx(ml[x * len] - ref), sum);
+#pragma unroll 8
+    for (int x = lane; x < S; x += 32) {
+      const float2 y = ml[warp * p.S + x];
+      sum = fmaf(y.y, exp2_approx(y.x - ref), sum);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
       s_norm[warp * 2] = ref;
-      s_norm[warp * 2 + 1] = sum == 0.f ? 0.f : 1.0f / sum;  // no rows: zeros
+      s_norm[warp * 2 + 1] = 1.0f / sum;
     }
   }
   __syncthreads();
-  const float* scores = p.scores + (int64_t)item * G * p.score_pitch;
-  float* wrow = wts + (int64_t)g * p.weight_stride;
-#pragma unroll 2
-  for (int64_t row = row0 + tid; row < row1; row += kJoinThreads)
-    wrow[row] += row_weight(scores + row, p.score_pitch, s_norm, G);
-  // outputs: 32 at a time, a warp for every eighth part
-  float* out = p.xb + ((int64_t)b * p.n_heads + (int64_t)g * G) * head_dim;
-  for (int i0 = share * 32; i0 < G * head_dim; i0 += shares * 32) {
-    const int i = i0 + lane, h = i / head_dim;  // G * head_dim is a multiple of 32
-    float acc = 0.f;
-#pragma unroll 4
-    for (int x = warp; x < S; x += kJoinThreads / 32)
-      acc = fmaf(part[x * len + i], exp2_approx(part[x * len + G * head_dim + h * 2] - s_norm[h * 2]), acc);
-    s_acc[warp][lane] = acc;
-    __syncthreads();
-    if (warp == 0) {
-      acc = 0.f;
+  if (share >= 0) {
 #pragma unroll
-      for (int x = 0; x < kJoinThreads / 32; ++x) acc += s_acc[x][lane];
-      out[i] = acc * s_norm[h * 2 + 1];
+    for (int r = 0; r < kPer; ++r) {
+      const int i = r * kJoinThreads + tid;
+      if (row0 + i < n) {
+        float x = 0.f;
+#pragma unroll
+        for (int h = 0; h < GP; ++h)
+          if (h < G) x = fmaf(exp2_approx(s[r][h] - s_norm[h * 2]), s_norm[h * 2 + 1], x);
+        wrow[i] = old[r] + x;
+      }
     }
-    __syncthreads();
+    return;
+  }
+  // outputs: a warp for every eighth part
+  const float ref = s_norm[out_head * 2];
+  const float* part = p.part + (int64_t)item * p.S * G * head_dim + out0 + lane;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int x = warp; x < S; x += kJoinThreads / 32)
+    acc = fmaf(__ldcg(part + (int64_t)x * G * head_dim),
+               exp2_approx(ml[out_head * p.S + x].x - ref), acc);
+  s_acc[warp][lane] = acc;
+  __syncthreads();
+  if (warp == 0) {
+    acc = 0.f;
+#pragma unroll
+    for (int x = 0; x < kJoinThreads / 32; ++x) acc += s_acc[x][lane];
+    p.xb[((int64_t)b * p.n_heads + (int64_t)g * G) * head_dim + out0 + lane] =
+        acc * s_norm[out_head * 2 + 1];
   }
 }
 
 // Rows of a part when a second kernel joins the parts, 0 when a cluster does.
-// Parts are sized for two waves of CTAs (three an SM) over a batch whose
-// sequences are all as long as the longest, and take at least 8 units a warp;
-// sequences too short for two such parts are left to a cluster (one launch
-// less, about 3 us).
-int32_t part_rows_for(int64_t items, int64_t max_rows, int unit, const DeviceInfo& dev) {
-  const int64_t step = 4 * unit, least = 8 * step;
-  int64_t rows = (max_rows * items + 6 * dev.sms - 1) / (6 * dev.sms);
+// A single sequence is cut into one wave of CTAs (three an SM).  A batch may be
+// ragged, and its CTAs are counted for the longest sequence: two waves, so that
+// half of them idle still leaves one (131,072 rows of one sequence: 64 us with one
+// wave, 68 with two; 16 sequences of 77 to 8191 rows: 41 and 30).  A part takes at
+// least 8 units a warp; sequences too short for two such parts are left to a
+// cluster (one launch less, about 3 us).
+int32_t part_rows_for(int32_t batch, int32_t n_kv, int64_t max_rows, int unit,
+                      const DeviceInfo& dev) {
+  const int64_t step = 4 * unit, least = 8 * step, items = (int64_t)batch * n_kv;
+  const int64_t ctas = (batch == 1 ? 3 : 6) * (int64_t)dev.sms;
+  int64_t rows = (max_rows * items + ctas - 1) / ctas;
   rows = std::max(least, (rows + step - 1) / step * step);
   return max_rows > rows ? (int32_t)rows : 0;
 }
@@ -833,20 +868,23 @@ int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t strea
   const int64_t items = (int64_t)r.batch * r.n_kv;
   if constexpr (!BLOCKS) {
     p.score_pitch = score_pitch_for(r.max_n_pos);
-    p.part_rows = part_rows_for(items, r.max_n_pos, U, dev);
+    p.part_rows = part_rows_for(r.batch, r.n_kv, r.max_n_pos, U, dev);
     if (p.part_rows) {
       const int64_t parts = ((int64_t)r.max_n_pos + p.part_rows - 1) / p.part_rows;
-      const int64_t shares = ((int64_t)r.max_n_pos + kJoinRows - 1) / kJoinRows;
+      const int32_t outs = (r.n_heads / r.n_kv) * HD / 32;
+      const int64_t shares = ((int64_t)r.max_n_pos + kJoinRows - 1) / kJoinRows + outs;
       if (items * parts > INT32_MAX || items * shares > INT32_MAX) {
         *err = "batch * n_kv_heads * max_n_pos too large";
         return GLA_ERR_NOT_SUPPORTED;
       }
-      p.part = r.scores + (size_t)(items * (r.n_heads / r.n_kv)) * p.score_pitch;
+      const int64_t heads = (int64_t)r.batch * r.n_heads;
+      p.part = r.scores + heads * p.score_pitch;
+      p.part_ml = reinterpret_cast<float2*>(p.part + heads * parts * r.head_dim);
       int rc = launch_shape<T, HD, BLOCKS, false>(p, items, (int)parts, stream, err);
       if (rc != GLA_OK) return rc;
       static std::atomic<uint64_t> attr_done{0};
       return launch_clusters(attend_join_kernel, (unsigned)(items * shares), kJoinThreads, 0, 1,
-                             attr_done, stream, "attention join", err, p, (int32_t)HD,
+                             attr_done, stream, "attention join", err, p, (int32_t)HD, outs,
                              (int32_t)shares);
     }
   }
@@ -874,7 +912,7 @@ int by_type(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream, 
 
 size_t attend_score_floats(const AttendRequest& r, const DeviceInfo& dev) {
   const int unit = r.dtype == GLA_DTYPE_F16 ? unit_rows<__half, 64>() : unit_rows<float, 64>();
-  const int64_t rows = part_rows_for((int64_t)r.batch * r.n_kv, r.max_n_pos, unit, dev);
+  const int64_t rows = part_rows_for(r.batch, r.n_kv, r.max_n_pos, unit, dev);
   const int64_t parts = rows ? ((int64_t)r.max_n_pos + rows - 1) / rows : 0;
   return (size_t)r.batch * r.n_heads *
          (size_t)(score_pitch_for(r.max_n_pos) + parts * (r.head_dim + 2));
