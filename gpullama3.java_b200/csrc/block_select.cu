@@ -29,6 +29,8 @@
 // where rank 0 selects alone with block barriers (a radix pass that every CTA
 // of the cluster took part in cost a cluster barrier of about 0.5 us each).
 // One launch, no global workspace.
+#include <algorithm>
+
 #include "cache_ops.cuh"
 
 namespace gla {
@@ -79,8 +81,8 @@ __device__ __forceinline__ float coefficient(float q, bool is_lo) {
 // kChunks 16-byte chunks, lo then hi, over kLanes lanes; a lane holds the
 // coefficients of its chunks in registers (at most 8 elements of GP heads) and
 // a lane group scores kBlk blocks at once, so that one reduce_scatter joins
-// them.  kBlk keeps the kernel at 128 registers: two CTAs an SM, one streams
-// while the other selects.
+// them.  The blocks come through a ring of each warp's own in shared memory
+// (cp.async), kStages steps deep: a step's latency is most of its time.
 template <class T, int HD, int GP>
 struct Shape {
   static constexpr int kPer = 16 / sizeof(T);
@@ -88,11 +90,26 @@ struct Shape {
   static constexpr int kLanes = kChunks > 16 ? 32 : 16;
   static constexpr int kCpl = (kChunks + kLanes - 1) / kLanes;
   static constexpr int kSub = 32 / kLanes;  // lane groups of a warp
-  static constexpr int kWant = GP <= 2 ? 8 / kCpl : (GP == 4 ? 4 : 4 / kCpl);
+  static constexpr int kWant = GP <= 2 ? 8 / kCpl : 4;
   static constexpr int kBlk = kWant * GP > kLanes ? kLanes / GP : kWant;  // a value a lane
   static constexpr int kVals = kBlk * GP;
+  static constexpr int kSlot = kSub * kBlk * kChunks * 16;  // bytes of a step
+  static constexpr int kStages = 72 * 1024 / (kWarps * kSlot) > 4 ? 4 : 72 * 1024 / (kWarps * kSlot);
+  static constexpr int kRing = kWarps * kStages * kSlot;
   static_assert(kCpl * kPer <= 8, "the error bound counts 8 terms a lane");
+  static_assert(kStages >= 2, "a step in flight beside the one at work");
 };
+
+// The ring and the 64-bit keys' upper words share their bytes.
+template <class T, int HD, int GP>
+size_t select_smem(int64_t max_nb) {
+  using Sh = Shape<T, HD, GP>;
+  return (size_t)std::max<int64_t>(Sh::kRing, max_nb * 4) + (size_t)max_nb * 4;
+}
+
+__device__ __forceinline__ void cp_async_chunk(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 
 // The FP64 score of one (block, kv head), by one warp: the larger product of
 // each channel, so that an infinite bound on the other side does not count
@@ -125,12 +142,14 @@ __global__ void __launch_bounds__(kThreads, 2)
                         const int32_t* __restrict__ n_pos, int32_t max_n_pos,
                         int32_t* __restrict__ block_ids, int32_t n_heads, int32_t n_kv,
                         int32_t br_shift, int32_t n_sel, int32_t n_first, int32_t n_last, int S,
-                        int32_t* __restrict__ status) {
+                        int32_t max_nb, int32_t* __restrict__ status) {
   using Sh = Shape<T, HD, GP>;
   constexpr int kPer = Sh::kPer, kLanes = Sh::kLanes, kCpl = Sh::kCpl, kBlk = Sh::kBlk;
+  constexpr int kStages = Sh::kStages;
   constexpr int kVals = Sh::kVals, kStep = kWarps * Sh::kSub * kBlk;
-  // rank 0's: one 64-bit slot a block; the FP32 keys use the low words first
-  extern __shared__ uint64_t s_slot[];
+  // the warps' rings, in rank 0 later the upper words of 64-bit keys; then rank 0's
+  // FP32 keys, later the lower words
+  extern __shared__ __align__(16) char s_dyn[];
   __shared__ SelectScratch sh;
   // rank 0's, of every warp of the cluster: M, the smallest and the largest key
   __shared__ float s_mag[16 * kWarps];
@@ -147,8 +166,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int G = n_heads / n_kv;
   pdl_wait();
   pdl_launch_dependents();
-  for (int i = tid; i < GP * HD; i += kThreads)
-    s_q[i] = i < G * HD ? __ldg(q + ((int64_t)b * n_heads + (int64_t)g * G) * HD + i) : 0.f;
+  // q, the length and the pointer are loaded side by side
+  constexpr int kQ = (GP * HD + kThreads - 1) / kThreads;
+  float qr[kQ];
+#pragma unroll
+  for (int i = 0; i < kQ; ++i) {
+    const int at = i * kThreads + tid;
+    qr[i] = at < G * HD ? __ldg(q + ((int64_t)b * n_heads + (int64_t)g * G) * HD + at) : 0.f;
+  }
   const int32_t n = clamped_rows(n_pos, b, max_n_pos, status);
   const T* bounds = bounds_ptrs[b];
   const bool ok = usable_ptrs(bounds, bounds, status);
@@ -167,22 +192,33 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int sub = lane / kLanes, sl = lane % kLanes;
   const int64_t row = (int64_t)n_kv * 2 * HD;
   const T* base = bounds + (int64_t)n_first * row + (int64_t)g * 2 * HD;
-  float4 x[kBlk][kCpl];
-  auto load = [&](int32_t j0) {
+  uint32_t* s_upper = reinterpret_cast<uint32_t*>(s_dyn);
+  uint32_t* s_lower = reinterpret_cast<uint32_t*>(s_dyn + max(Sh::kRing, max_nb * 4));
+  const uint32_t ring = smem_u32(s_dyn) + warp * (kStages * Sh::kSlot) + sub * (Sh::kSlot / Sh::kSub);
+  auto fetch = [&](int s, int32_t jw) {  // blocks jw + sub * kBlk + 0 .. kBlk - 1
+    if (jw < hi) {
 #pragma unroll
-    for (int i = 0; i < kBlk; ++i) {
-      const T* src = base + (int64_t)min(j0 + i, hi - 1) * row;
+      for (int i = 0; i < kBlk; ++i) {
+        const T* src = base + (int64_t)min(jw + sub * kBlk + i, hi - 1) * row;
 #pragma unroll
-      for (int c = 0; c < kCpl; ++c) {
-        const int chunk = sl + c * kLanes;
-        x[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (chunk < Sh::kChunks) x[i][c] = __ldg(reinterpret_cast<const float4*>(src) + chunk);
+        for (int c = 0; c < kCpl; ++c) {
+          const int chunk = sl + c * kLanes;
+          if (chunk < Sh::kChunks)
+            cp_async_chunk(ring + s * Sh::kSlot + (i * Sh::kChunks + chunk) * 16,
+                           reinterpret_cast<const float4*>(src) + chunk);
+        }
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   const int32_t w0 = lo + warp * Sh::kSub * kBlk;  // the warp's first block
-  if (w0 < hi) load(w0 + sub * kBlk);  // in flight while the coefficients are set up
+  // in flight while the coefficients are set up
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) fetch(s, w0 + s * kStep);
   cluster_arrive(S);
+#pragma unroll
+  for (int i = 0; i < kQ; ++i)
+    if (i * kThreads + tid < GP * HD) s_q[i * kThreads + tid] = qr[i];
   __syncthreads();
   float co[kCpl * kPer][GP];
 #pragma unroll
@@ -197,47 +233,59 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 
   // keys, M and the keys' range go to rank 0's shared memory
-  uint32_t* key0 = reinterpret_cast<uint32_t*>(
-      S > 1 ? const_cast<uint64_t*>(cluster_peer(s_slot, 0)) : s_slot);
+  uint32_t* key0 = S > 1 ? const_cast<uint32_t*>(cluster_peer(s_lower, 0)) : s_lower;
   cluster_wait(S);  // rank 0 is running: its shared memory may be written
   float big = 0.f;
-  bool strange = false;  // a NaN bound, which a maximum would drop
+  bool strange = false;  // a NaN bound (its scores are NaN; a maximum would drop it)
   uint32_t kmin = ~0u, kmax = 0;
-  for (int32_t jw = w0; jw < hi; jw += kStep) {
-    const int32_t j0 = jw + sub * kBlk;
-    float acc[kVals];
+  for (int32_t jw0 = w0; jw0 < hi; jw0 += kStages * kStep) {
 #pragma unroll
-    for (int i = 0; i < kBlk; ++i) {
+    for (int st = 0; st < kStages; ++st) {
+      const int32_t jw = jw0 + st * kStep, j0 = jw + sub * kBlk;
+      if (jw >= hi) break;
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+      __syncwarp();
+      float acc[kVals];
 #pragma unroll
-      for (int h = 0; h < GP; ++h) acc[i * GP + h] = 0.f;
+      for (int i = 0; i < kBlk; ++i) {
 #pragma unroll
-      for (int c = 0; c < kCpl; ++c) {
+        for (int h = 0; h < GP; ++h) acc[i * GP + h] = 0.f;
 #pragma unroll
-        for (int p = 0; p < kPer; ++p) {
-          const float y = (float)reinterpret_cast<const T*>(&x[i][c])[p];
-          big = fmaxf(big, fabsf(y));
-          strange |= y != y;
+        for (int c = 0; c < kCpl; ++c) {
+          const int chunk = sl + c * kLanes;
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (chunk < Sh::kChunks)
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                         : "r"(ring + st * Sh::kSlot + (i * Sh::kChunks + chunk) * 16));
 #pragma unroll
-          for (int h = 0; h < GP; ++h)
-            acc[i * GP + h] = fmaf(co[c * kPer + p][h], y, acc[i * GP + h]);
+          for (int p = 0; p < kPer; ++p) {
+            const float y = (float)reinterpret_cast<const T*>(&x)[p];
+            big = fmaxf(big, fabsf(y));
+#pragma unroll
+            for (int h = 0; h < GP; ++h)
+              acc[i * GP + h] = fmaf(co[c * kPer + p][h], y, acc[i * GP + h]);
+          }
         }
       }
-    }
-    if (jw + kStep < hi) load(j0 + kStep);
-    const float s = reduce_scatter<kVals, kLanes>(acc, sl);
-    // lane sl holds value sl >> kRep: block value / GP, head value % GP
-    constexpr int kRep = ilog2(kLanes) - ilog2(kVals);
-    const int val = sl >> kRep;
-    const int h = val % GP;
-    uint32_t key = h < G ? order_key(s) : 0;
+      __syncwarp();  // read out by every lane
+      fetch(st, jw + kStages * kStep);
+      const float s = reduce_scatter<kVals, kLanes>(acc, sl);
+      // lane sl holds value sl >> kRep: block value / GP, head value % GP
+      constexpr int kRep = ilog2(kLanes) - ilog2(kVals);
+      const int val = sl >> kRep;
+      const int h = val % GP;
+      strange |= s != s;
+      uint32_t key = h < G ? order_key(s) : 0;
 #pragma unroll
-    for (int m = (GP << kRep) >> 1; m >= (1 << kRep) && m > 0; m >>= 1)
-      key = max(key, __shfl_xor_sync(0xffffffffu, key, m));
-    const int32_t j = j0 + val / GP;
-    if (j < hi) {
-      kmin = min(kmin, key);
-      kmax = max(kmax, key);
-      if (h == 0 && (sl & ((1 << kRep) - 1)) == 0) key0[2 * (int64_t)j] = key;
+      for (int m = (GP << kRep) >> 1; m >= (1 << kRep) && m > 0; m >>= 1)
+        key = max(key, __shfl_xor_sync(0xffffffffu, key, m));
+      const int32_t j = j0 + val / GP;
+      if (j < hi) {
+        kmin = min(kmin, key);
+        kmax = max(kmax, key);
+        if (h == 0 && (sl & ((1 << kRep) - 1)) == 0) key0[j] = key;
+      }
     }
   }
   // M of this warp's blocks (its lane groups see different blocks: their maximum counts)
@@ -276,8 +324,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   for (int i = tid; i < n_first + n_last; i += kThreads)
     ids[i < n_first ? i : pick + i] = i < n_first ? i : nc + i;
   ids += n_first;
-  uint32_t* key32 = reinterpret_cast<uint32_t*>(s_slot);
-  auto key_of = [&](int32_t i) { return key32[2 * (int64_t)i]; };
+  auto key_of = [&](int32_t i) { return s_lower[i]; };
   auto emit = [&](int32_t i, uint32_t at) { ids[at] = n_first + i; };
   mag = 0.f;
   kmin = ~0u;
@@ -291,9 +338,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   for (int m = 16; m > 0; m >>= 1) mag = fmaxf(mag, __shfl_xor_sync(0xffffffffu, mag, m));
   kmin = __reduce_min_sync(0xffffffffu, kmin);
   kmax = __reduce_max_sync(0xffffffffu, kmax);
-  const int bits = 32 - __clz((int)(kmax - kmin));
   const Threshold<uint32_t> th = find_threshold<kThreads, uint32_t>(
-      sh, 1, nc, (uint32_t)pick, kmin, bits > 8 ? bits - 8 : 0, key_of);
+      sh, 1, nc, (uint32_t)pick, kmin, kmax, key_of);
   // the lowest chosen and the highest other key
   uint32_t least = ~0u, most = 0;
 #pragma unroll 4
@@ -347,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       int32_t before = 0;
       for (int32_t i = 0; i < near_n; ++i)
         before += s_near_key[i] > k || (s_near_key[i] == k && s_near[i] < me);
-      key32[2 * (int64_t)me] = before < wanted ? ~0u : 0u;
+      s_lower[me] = before < wanted ? ~0u : 0u;
     }
     __syncthreads();
     // sure ones exceed `most`; the near ones no longer do unless they are wanted
@@ -367,12 +413,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       key64 = exact_key<T, HD>(base + (int64_t)i * row, s_q, G, lane);
     }
     __syncwarp();
-    if (lane == 0) s_slot[i] = key64;
+    if (lane == 0) {
+      s_lower[i] = (uint32_t)key64;
+      s_upper[i] = (uint32_t)(key64 >> 32);
+    }
   }
   __syncthreads();
-  auto slot_of = [&](int32_t i) { return s_slot[i]; };
+  auto slot_of = [&](int32_t i) { return (uint64_t)s_upper[i] << 32 | s_lower[i]; };
   const Threshold<uint64_t> th64 = find_threshold<kThreads, uint64_t>(
-      sh, 1, nc, (uint32_t)pick, (uint64_t)0, 56, slot_of);
+      sh, 1, nc, (uint32_t)pick, (uint64_t)0, ~(uint64_t)0, slot_of);
   emit_chosen<kThreads, uint64_t>(sh, 1, 0, nc, th64, slot_of, emit);
 }
 
@@ -397,10 +446,10 @@ int launch_select(const SelectRequest& r, const DeviceInfo& dev, cudaStream_t st
     return GLA_ERR_NOT_SUPPORTED;
   }
   return launch_clusters(block_select_kernel<T, HD, GP>, (unsigned)(items * S), kThreads,
-                         (size_t)max_nb * 8, S, attr_done, stream, "block selection", err, r.q,
+                         select_smem<T, HD, GP>(max_nb), S, attr_done, stream, "block selection", err, r.q,
                          reinterpret_cast<const T* const*>(r.bounds_ptrs), r.n_pos, r.max_n_pos,
                          r.block_ids, r.n_heads, r.n_kv, br_shift, r.n_sel, r.n_first, r.n_last, S,
-                         r.status);
+                         (int32_t)max_nb, r.status);
 }
 
 template <class T, int HD>

@@ -148,17 +148,16 @@ __device__ __forceinline__ float key_score(uint32_t key) {
 // contiguous index range, ranges ascending with the rank; 0 < k < all keys.
 // The keys are walked once a pass: they belong in shared memory.
 //
-// find_threshold: radix selection, 8 bits a pass.  Every CTA counts the digits
-// of its keys in the range found so far, one cluster barrier publishes the
-// counts, and every CTA adds all ranks' counts itself (so the ranks agree
-// without a second barrier; two count buffers keep a fast rank from clearing
-// what a slow one still reads).  A pass whose bin is taken whole ends the
-// search.  The first range, [base, base + 256 << shift), holds every key; a
-// caller that knows the smallest and largest key passes a range that fits
-// them: full-width digits would put nearly all scores into a few bins first.
-// emit_chosen: each warp, which owns a contiguous share of the CTA's keys,
-// counts what it holds above and at the threshold, and after one more barrier
-// writes its chosen indices, so the list ascends with no barrier inside:
+// find_threshold: radix selection, 8 bits a pass over the range [kmin, kmax] of the
+// keys (key_range finds it: full-width digits would put nearly all scores into a few
+// bins first and take more passes).  Every CTA counts the digits of its keys in the range found so far, one cluster
+// barrier publishes the counts, and every CTA adds all ranks' counts itself (so the
+// ranks agree without a second barrier; two count buffers keep a fast rank from
+// clearing what a slow one still reads).  A pass whose bin is taken whole ends the
+// search.
+// emit_chosen: each warp, which owns a contiguous share of the CTA's keys, counts
+// what it holds above and at the threshold, and after one more barrier writes its
+// chosen indices, so the list ascends with no barrier inside:
 // emit(local index, position in the list of all chosen).
 // ---------------------------------------------------------------------------
 constexpr int kSelectWarps = 16;  // at most
@@ -169,7 +168,11 @@ struct SelectScratch {
   uint32_t above[kSelectWarps];      // of each warp's share: keys above the threshold
   uint32_t at[kSelectWarps];         // and at it
   uint32_t counts[2];                // of the CTA's share
+  uint32_t low[kSelectWarps], high[kSelectWarps];  // each warp's smallest and largest key
 };
+
+__device__ __forceinline__ int bit_count(uint32_t x) { return 32 - __clz((int)x); }
+__device__ __forceinline__ int bit_count(uint64_t x) { return 64 - __clzll((long long)x); }
 
 template <class Key>
 struct Threshold {
@@ -180,18 +183,43 @@ struct Threshold {
   __device__ __forceinline__ bool above(Key k) const { return k >= lo && k - lo > span; }
 };
 
+// The smallest and the largest of the cluster's keys from those of each thread.
+template <int THREADS>
+__device__ __forceinline__ void key_range(SelectScratch& sh, int S, uint32_t* kmin, uint32_t* kmax) {
+  constexpr int W = THREADS / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t lo = __reduce_min_sync(0xffffffffu, *kmin), hi = __reduce_max_sync(0xffffffffu, *kmax);
+  if (lane == 0) {
+    sh.low[warp] = lo;
+    sh.high[warp] = hi;
+  }
+  cluster_barrier(S);
+  lo = ~0u;
+  hi = 0;
+  if (lane < W) {
+#pragma unroll 4
+    for (int r = 0; r < S; ++r) {
+      lo = min(lo, S == 1 ? sh.low[lane] : *cluster_peer(&sh.low[lane], r));
+      hi = max(hi, S == 1 ? sh.high[lane] : *cluster_peer(&sh.high[lane], r));
+    }
+  }
+  *kmin = __reduce_min_sync(0xffffffffu, lo);
+  *kmax = __reduce_max_sync(0xffffffffu, hi);
+}
+
 template <int THREADS, class Key, class KeyFn>
 __device__ __forceinline__ Threshold<Key> find_threshold(SelectScratch& sh, int S, int32_t n_local,
-                                                         uint32_t k, Key base, int shift,
+                                                         uint32_t k, Key kmin, Key kmax,
                                                          KeyFn key) {
   static_assert(THREADS >= 256 && THREADS % 32 == 0, "one thread per histogram bin");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t need = k;  // of the keys in the range
   bool whole = false;
   int buf = 0;
-  Key span = ~(Key)0;  // the range is [base, base + span]
   for (int i = tid; i < 512; i += THREADS) (&sh.hist[0][0])[i] = 0;
   __syncthreads();
+  Key base = kmin, span = kmax - kmin;  // the range is [base, base + span]
+  int shift = bit_count(span) > 8 ? bit_count(span) - 8 : 0;
   for (;; buf ^= 1) {
 #pragma unroll 4
     for (int32_t i = tid; i < n_local; i += THREADS) {
@@ -275,36 +303,42 @@ __device__ __forceinline__ void emit_chosen(SelectScratch& sh, int S, int rank, 
     }
     cluster_barrier(S);
   }
-  // keys chosen, and keys at the threshold, before this warp's share
-  uint32_t out = 0, at_before = 0;
-  auto skip = [&](uint32_t a, uint32_t e) {
-    const uint32_t room = need > at_before ? need - at_before : 0;
-    out += a + (e < room ? e : room);
-    at_before += e;
-  };
-  if (S > 1)
-    for (int r = 0; r < rank; ++r) {
-      const uint32_t* c = cluster_peer(sh.counts, r);
-      skip(c[0], c[1]);
-    }
-#pragma unroll
-  for (int w = 0; w < W - 1; ++w)
-    if (w < warp) skip(sh.above[w], sh.at[w]);
-  const unsigned below = (1u << lane) - 1;
-#pragma unroll 4
-  for (int32_t i0 = w_lo; i0 < w_hi; i0 += 32) {
-    const int32_t i = i0 + lane;
-    const bool in = i < w_hi;
-    const Key kv = key(in ? i : w_lo);
-    const bool eq = in && th.at(kv);
-    const unsigned beq = __ballot_sync(0xffffffffu, eq);
-    const bool take = (in && th.above(kv)) || (eq && at_before + __popc(beq & below) < need);
-    const unsigned bt = __ballot_sync(0xffffffffu, take);
-    if (take) emit(i, out + __popc(bt & below));
-    out += __popc(bt);
-    at_before += __popc(beq);
+  // keys above, and at the threshold, before this warp's share
+  uint32_t before = lane < warp ? sh.above[lane % W] : 0;
+  uint32_t at_before = lane < warp ? sh.at[lane % W] : 0;
+  if (S > 1 && lane < rank) {  // a cluster has at most 16 CTAs
+    const uint32_t* c = cluster_peer(sh.counts, lane);
+    before += c[0];
+    at_before += c[1];
   }
-  cluster_barrier(S);  // no CTA leaves while another still reads its counts
+  before = __reduce_add_sync(0xffffffffu, before);
+  at_before = __reduce_add_sync(0xffffffffu, at_before);
+  uint32_t out = before + (at_before < need ? at_before : need);
+  const unsigned below = (1u << lane) - 1;
+  if (th.whole) {
+#pragma unroll 4
+    for (int32_t i0 = w_lo; i0 < w_hi; i0 += 32) {
+      const int32_t i = i0 + lane;
+      const bool take = i < w_hi && key(min(i, w_hi - 1)) >= th.lo;
+      const unsigned bt = __ballot_sync(0xffffffffu, take);
+      if (take) emit(i, out + __popc(bt & below));
+      out += __popc(bt);
+    }
+  } else {
+    for (int32_t i0 = w_lo; i0 < w_hi; i0 += 32) {
+      const int32_t i = i0 + lane;
+      const bool in = i < w_hi;
+      const Key kv = key(in ? i : w_lo);
+      const bool eq = in && th.at(kv);
+      const unsigned beq = __ballot_sync(0xffffffffu, eq);
+      const bool take = (in && th.above(kv)) || (eq && at_before + __popc(beq & below) < need);
+      const unsigned bt = __ballot_sync(0xffffffffu, take);
+      if (take) emit(i, out + __popc(bt & below));
+      out += __popc(bt);
+      at_before += __popc(beq);
+    }
+  }
+  if (S > 1) cluster_barrier(S);  // no CTA leaves while another still reads its counts
 }
 
 // Contiguous share [lo, hi) of n items for CTA `rank` of S.

@@ -50,15 +50,27 @@ __global__ void __launch_bounds__(kSelThreads)
   int32_t lo, hi;
   share_of(older, S, rank, &lo, &hi);
   const float* mine = w + (int64_t)g * weight_stride + lo;
-  const int32_t staged = min(hi - lo, key_cap);
-#pragma unroll 8
-  for (int32_t i = tid; i < staged; i += kSelThreads) s_key[i] = order_key(__ldcg(mine + i));
-  __syncthreads();
-  auto key = [&](int32_t i) { return i < staged ? s_key[i] : order_key(__ldcg(mine + i)); };
-  const Threshold<uint32_t> th =
-      find_threshold<kSelThreads, uint32_t>(sh, S, hi - lo, (uint32_t)pick, 0u, 24, key);
-  emit_chosen<kSelThreads, uint32_t>(sh, S, rank, hi - lo, th, key,
-                                     [&](int32_t i, uint32_t at) { out[at] = lo + i; });
+  const bool fits = (older + S - 1) / S <= key_cap;  // (not so past 16 CTAs' shared memory)
+  uint32_t kmin = ~0u, kmax = 0;
+#pragma unroll 4
+  for (int32_t i = tid; i < hi - lo; i += kSelThreads) {
+    const uint32_t k = order_key(__ldcg(mine + i));
+    if (fits) s_key[i] = k;
+    kmin = min(kmin, k);
+    kmax = max(kmax, k);
+  }
+  key_range<kSelThreads>(sh, S, &kmin, &kmax);  // (a barrier: the keys are staged)
+  auto select = [&](auto key) {
+    const Threshold<uint32_t> th = find_threshold<kSelThreads, uint32_t>(
+        sh, S, hi - lo, (uint32_t)pick, kmin, kmax, key);
+    emit_chosen<kSelThreads, uint32_t>(sh, S, rank, hi - lo, th, key,
+                                       [&](int32_t i, uint32_t at) { out[at] = lo + i; });
+  };
+  // the ranks' shares differ by rounding alone, and every rank takes the same way
+  if (fits)
+    select([&](int32_t i) { return s_key[i]; });
+  else
+    select([&](int32_t i) { return order_key(__ldcg(mine + i)); });
 }
 
 // Kept rows of one kv head to another cache: thread = (row, 16-byte chunk).
@@ -269,11 +281,12 @@ int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stre
                  std::string* err) {
   static std::atomic<uint64_t> attr_done{0};
   const int64_t items = (int64_t)r.batch * r.n_kv;
-  // a CTA for every 2048 weights, as long as that does not exceed the device; and
-  // enough for the keys to fit shared memory (past 16 CTAs the rest is read again a pass)
+  // a CTA for every 8192 weights (a cluster's barriers cost about as much as walking
+  // that many), as long as that does not exceed four CTAs an SM; and enough for the
+  // keys to fit shared memory (past 16 CTAs the rest is read again a pass)
   const int64_t most_keys = (dev.smem_optin - 8 * 1024) / 4;
   int S = 1;
-  while (S < 16 && ((items * S < dev.sms && r.max_n_pos > (int64_t)2048 * S) ||
+  while (S < 16 && ((items * S < 3 * dev.sms && r.max_n_pos > (int64_t)8192 * S) ||
                     r.max_n_pos > most_keys * S))
     S *= 2;
   const int32_t key_cap =

@@ -58,13 +58,14 @@ constexpr size_t kEpochOffset = 64;
 // Makes the context's device current for the duration of a call.
 struct DeviceGuard {
   int prev = -1;
+  int device;
   bool ok = true;
-  explicit DeviceGuard(int dev) {
+  explicit DeviceGuard(int dev) : device(dev) {
     if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
     if (prev != dev) ok = cudaSetDevice(dev) == cudaSuccess;
   }
   ~DeviceGuard() {
-    if (prev >= 0) cudaSetDevice(prev);
+    if (prev >= 0 && prev != device) cudaSetDevice(prev);
   }
 };
 

@@ -155,17 +155,15 @@ struct AttendParams {
   int32_t* status;
 };
 
-// Where unit u's rows start, or -1 if it has none.  kUnitShift: log2 of the
-// rows of a unit.
+// Where unit u's rows start, or -1 if it has none, from the id of its block (all
+// rows: no id).  kUnitShift: log2 of the rows of a unit.
 template <bool BLOCKS, int kUnitShift>
-__device__ __forceinline__ int32_t unit_row(const AttendParams& p, const int32_t* ids, int32_t u,
-                                            int32_t n) {
+__device__ __forceinline__ int32_t unit_row(int32_t br_shift, int32_t id, int32_t u, int32_t n) {
   int64_t row;
   if constexpr (BLOCKS) {
-    const int shift = p.br_shift - kUnitShift;  // units of a block, log2
-    const int32_t id = __ldg(ids + (u >> shift));
+    const int shift = br_shift - kUnitShift;  // units of a block, log2
     if (id < 0) return -1;
-    row = ((int64_t)id << p.br_shift) + ((int64_t)(u & ((1 << shift) - 1)) << kUnitShift);
+    row = ((int64_t)id << br_shift) + ((int64_t)(u & ((1 << shift) - 1)) << kUnitShift);
   } else {
     row = (int64_t)u << kUnitShift;
   }
@@ -241,24 +239,31 @@ struct WarpF16 {
   float factor;             // score = product * factor (log2 units)
 
   // q of the group's heads, scaled and split into shared memory, then to registers.
+  static constexpr int kQBytes = 16 * kPitch + 32;
+
   template <int W>
   __device__ __forceinline__ void init(const float* q, int G, float scale_log2, char* scratch,
-                                       uint4*, int warp, int lane) {
+                                       int warp, int lane) {
     __half* s_q = reinterpret_cast<__half*>(scratch);                 // [16][HD + 8]
     float* s_f = reinterpret_cast<float*>(scratch + 16 * kPitch);     // [8]
-    for (int h = warp; h < 8; h += W) {  // one head a warp at a time
-      float x[HD / 32], big = 0.f;
+    float x[8 / W][HD / 32];
 #pragma unroll
-      for (int i = 0; i < HD / 32; ++i) {
-        x[i] = h < G ? q[(int64_t)h * HD + i * 32 + lane] : 0.f;
-        big = fmaxf(big, fabsf(x[i]));
-      }
+    for (int j = 0; j < 8 / W; ++j)  // one head a warp at a time
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i)
+        x[j][i] = warp + j * W < G ? q[(int64_t)(warp + j * W) * HD + i * 32 + lane] : 0.f;
+#pragma unroll
+    for (int j = 0; j < 8 / W; ++j) {
+      const int h = warp + j * W;
+      float big = 0.f;
+#pragma unroll
+      for (int i = 0; i < HD / 32; ++i) big = fmaxf(big, fabsf(x[j][i]));
 #pragma unroll
       for (int s = 16; s > 0; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
       const int e = (big > 0.f && big < INFINITY) ? ilogbf(big) : 0;
 #pragma unroll
       for (int i = 0; i < HD / 32; ++i) {
-        const float y = scalbnf(x[i], -e);
+        const float y = scalbnf(x[j][i], -e);
         const __half hi = __float2half_rn(y);
         s_q[h * (HD + 8) + i * 32 + lane] = hi;
         s_q[(h + 8) * (HD + 8) + i * 32 + lane] = __float2half_rn(y - __half2float(hi));
@@ -271,7 +276,6 @@ struct WarpF16 {
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) ldmatrix_x4(qa[ks], base + ks * 32);
     factor = s_f[lane >> 2];
-    __syncthreads();
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i)
 #pragma unroll
@@ -282,7 +286,7 @@ struct WarpF16 {
 
   template <bool WEIGHTS>
   __device__ __forceinline__ void step(uint32_t slot, int rows, float* scores, int64_t pitch,
-                                       int G, const uint4*, int lane) {
+                                       int G, const char*, int lane) {
     float s[2][2];
     const int sub = lane >> 3, in = lane & 7;
 #pragma unroll
@@ -385,9 +389,12 @@ struct WarpF32 {
   float m, l;          // head lane / 4; l: this lane's share of the sum
   float factor;
 
+  static constexpr int kQBytes = HD / 8 * 32 * 16;
+
   template <int W>
-  __device__ __forceinline__ void init(const float* q, int G, float scale_log2, char*, uint4* s_q,
+  __device__ __forceinline__ void init(const float* q, int G, float scale_log2, char* scratch,
                                        int warp, int lane) {
+    uint4* s_q = reinterpret_cast<uint4*>(scratch);
     // fragment of step ks: (hi, lo) of channels 8 ks + (lane & 3) and + 4 of head lane / 4
     for (int i = warp * 32 + lane; i < HD / 8 * 32; i += W * 32) {
       const int l = i & 31, h = l >> 2, ch = (i >> 5) * 8 + (l & 3);
@@ -413,7 +420,8 @@ struct WarpF32 {
 
   template <bool WEIGHTS>
   __device__ __forceinline__ void step(uint32_t slot, int rows, float* scores, int64_t pitch,
-                                       int G, const uint4* s_q, int lane) {
+                                       int G, const char* scratch, int lane) {
+    const uint4* s_q = reinterpret_cast<const uint4*>(scratch);
     // scores: accumulators of 32 channels each, added in FP32 (see WarpF16)
     float c[HD / 32][4];
     const uint32_t kbase = slot + (lane >> 2) * kPitch + (lane & 3) * 4;
@@ -541,7 +549,11 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   constexpr int kSlot = slot_bytes<T, HD>();
   extern __shared__ __align__(16) char s_ring[];
   __shared__ float s_ml[GP * 2];
-  __shared__ uint4 s_q[sizeof(T) == 4 ? HD / 8 * 32 : 1];  // FP32: q's fragments
+  __shared__ __align__(16) char s_q[Warp::kQBytes];  // q, split
+  // wide CTAs of a cluster: what the others send, this rank's share of their outputs
+  // [S][share] and all their (m, l) [S][GP][2]
+  __shared__ float s_recv[WIDE ? GP * HD + 16 : 1];
+  __shared__ float s_recv_ml[WIDE ? 16 * GP * 2 : 1];
   __shared__ float s_norm[GP * 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int S = p.S;
@@ -577,9 +589,6 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   float* scores = WEIGHTS ? p.scores + (int64_t)item * G * p.score_pitch : nullptr;
 
   const uint32_t ring = smem_u32(s_ring) + warp * (kStages * kSlot);
-  Warp w;
-  w.template init<kWarps>(p.q + ((int64_t)b * p.n_heads + (int64_t)g * G) * HD, G, p.scale_log2,
-                          s_ring, s_q, warp, lane);
   const uint64_t policy = WEIGHTS ? l2_evict_first_policy() : 0;
 
   // unit i of this warp is first + i * stride; its ring slot i % kStages.  A slot
@@ -587,17 +596,29 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   // ring's other units are under way too.
   const int32_t mine = units > first ? (units - first - 1) / stride + 1 : 0;
   int32_t row_of[kStages];
-  auto fetch = [&](int s, int32_t i) {
+  // ids are loaded a step before the rows they name
+  auto id_of = [&](int32_t i) {
+    return BLOCKS && i < mine ? __ldg(ids + ((first + i * stride) >> (p.br_shift - kShift))) : -1;
+  };
+  auto fetch = [&](int s, int32_t i, int32_t id) {
     row_of[s] = -1;
     if (i < mine) {
-      row_of[s] = unit_row<BLOCKS, kShift>(p, ids, first + i * stride, n);
+      row_of[s] = unit_row<BLOCKS, kShift>(p.br_shift, id, first + i * stride, n);
       if (row_of[s] >= 0)
         load_unit<T, HD, U, WEIGHTS>(ring + s * kSlot, k, v, p.kv_bytes, row_of[s], n, policy, lane);
     }
     cp_async_commit();
   };
+  int32_t id[kStages + 1];
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) fetch(s, s);
+  for (int s = 0; s <= kStages; ++s) id[s] = id_of(s);
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) fetch(s, s, id[s]);
+  int32_t next_id = id[kStages];
+  if (WIDE) cluster_arrive(S);
+  Warp w;  // while the first units are under way
+  w.template init<kWarps>(p.q + ((int64_t)b * p.n_heads + (int64_t)g * G) * HD, G, p.scale_log2,
+                          s_q, warp, lane);
   for (int32_t i0 = 0; i0 < mine; i0 += kStages) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) {
@@ -608,7 +629,8 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
           w.template step<WEIGHTS>(ring + s * kSlot, n - row_of[s], scores + row_of[s],
                                    p.score_pitch, G, s_q, lane);
         __syncwarp();  // and read out by every lane
-        fetch(s, i0 + s + kStages);
+        fetch(s, i0 + s + kStages, next_id);
+        next_id = id_of(i0 + s + kStages + 1);
       }
     }
   }
@@ -622,73 +644,96 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   float* s_o = sml + kWarps * GP * 2;
   w.store(so + warp * GP * HD, sml + warp * GP * 2, lane);
   __syncthreads();
-  float* part = p.part + ((int64_t)item * S + rank) * G * HD;
-  for (int i = tid; i < GP * HD; i += kThreads) {
-    const int h = i / HD;
-    float top = -INFINITY;
+  auto cta_ml = [&](int h) {
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sml[(x * GP + h) * 2]);
     const float ref = top == -INFINITY ? 0.f : top;
-    float acc = 0.f, sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < kWarps; ++x) {
-      const float e = exp2_approx(sml[(x * GP + h) * 2] - ref);
-      acc = fmaf(so[x * GP * HD + i], e, acc);
-      sum = fmaf(sml[(x * GP + h) * 2 + 1], e, sum);
-    }
-    if (WEIGHTS && p.part) {  // joined by attend_join_kernel
-      if (h < G) {
-        part[i] = acc;
-        if (i == h * HD) p.part_ml[((int64_t)item * G + h) * S + rank] = make_float2(top, sum);
-      }
-      continue;
-    }
-    s_o[i] = acc;
-    if (i == h * HD) {
-      s_ml[h * 2] = top;
-      s_ml[h * 2 + 1] = sum;
-    }
-  }
-  if (WEIGHTS && p.part) return;
-  cluster_barrier(S);
-
-  // CTAs -> result: each rank joins its share of the G x HD outputs
-  float* out = p.xb + ((int64_t)b * p.n_heads + (int64_t)g * G) * HD;
-  for (int i = rank * kThreads + tid; i < G * HD; i += S * kThreads) {
-    const int h = i / HD;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int x = 0; x < S; ++x) top = fmaxf(top, S == 1 ? s_ml[h * 2] : *cluster_peer(&s_ml[h * 2], x));
+    for (int x = 0; x < kWarps; ++x)
+      sum = fmaf(sml[(x * GP + h) * 2 + 1], exp2_approx(sml[(x * GP + h) * 2] - ref), sum);
+    return make_float2(top, sum);
+  };
+  auto cta_o = [&](int i, float top) {
     const float ref = top == -INFINITY ? 0.f : top;
-    float acc = 0.f, sum = 0.f;
+    float acc = 0.f;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x)
+      acc = fmaf(so[x * GP * HD + i], exp2_approx(sml[(x * GP + i / HD) * 2] - ref), acc);
+    return acc;
+  };
+  // the outputs of a list of (o, m, l): o_of(x) and ml_of(x, h) of rank x
+  float* out = p.xb + ((int64_t)b * p.n_heads + (int64_t)g * G) * HD;
+  auto joined_ml = [&](int h, auto ml_of) {
+    float top = -INFINITY, sum = 0.f;
 #pragma unroll 4
-    for (int x = 0; x < S; ++x) {
-      const float* ml = S == 1 ? &s_ml[h * 2] : cluster_peer(&s_ml[h * 2], x);
-      const float* ox = S == 1 ? &s_o[i] : cluster_peer(&s_o[i], x);
-      const float e = exp2_approx(ml[0] - ref);
-      acc = fmaf(*ox, e, acc);
-      sum = fmaf(ml[1], e, sum);
-    }
-    // no row at all: zeros (sum is 0 only then: the largest weight is 1, or NaN)
-    out[i] = sum == 0.f ? 0.f : acc / sum;
-  }
-  if constexpr (WEIGHTS) {
+    for (int x = 0; x < S; ++x) top = fmaxf(top, ml_of(x, h)[0]);
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+    for (int x = 0; x < S; ++x) sum = fmaf(ml_of(x, h)[1], exp2_approx(ml_of(x, h)[0] - ref), sum);
+    return make_float2(ref, sum);
+  };
+  auto joined_o = [&](int i, auto o_of, auto ml_of) {
+    const int h = i / HD;
+    const float2 rs = joined_ml(h, ml_of);
+    float acc = 0.f;
+#pragma unroll 4
+    for (int x = 0; x < S; ++x) acc = fmaf(*o_of(x), exp2_approx(ml_of(x, h)[0] - rs.x), acc);
+    // no row at all: zeros (the sum is 0 only then: the largest weight is 1, or NaN)
+    out[i] = rs.y == 0.f ? 0.f : acc / rs.y;
+  };
+  auto norm_of = [&](auto ml_of) {  // p = 2^(s - ref) / sum
     if (tid < GP) {
-      float top = -INFINITY, sum = 0.f;
-#pragma unroll 4
-      for (int x = 0; x < S; ++x)
-        top = fmaxf(top, S == 1 ? s_ml[tid * 2] : *cluster_peer(&s_ml[tid * 2], x));
-      const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-      for (int x = 0; x < S; ++x) {
-        const float* ml = S == 1 ? &s_ml[tid * 2] : cluster_peer(&s_ml[tid * 2], x);
-        sum = fmaf(ml[1], exp2_approx(ml[0] - ref), sum);
-      }
-      s_norm[tid * 2] = ref;  // p = 2^(s - ref) / sum
-      s_norm[tid * 2 + 1] = 1.0f / sum;
+      const float2 rs = joined_ml(tid, ml_of);
+      s_norm[tid * 2] = rs.x;
+      s_norm[tid * 2 + 1] = 1.0f / rs.y;
     }
+    __syncthreads();
+  };
+  if (WEIGHTS && p.part) {  // joined by attend_join_kernel
+    float* part = p.part + ((int64_t)item * S + rank) * G * HD;
+    for (int i = tid; i < G * HD; i += kThreads) part[i] = cta_o(i, cta_ml(i / HD).x);
+    if (tid < G) p.part_ml[((int64_t)item * G + tid) * S + rank] = cta_ml(tid);
+    return;
   }
-  cluster_barrier(S);  // no CTA leaves while another reads its shared memory
+  if (WIDE && S > 1) {
+    // every rank sends each other one its share: one barrier, and local reads behind it
+    const int share = (G * HD + S - 1) / S;
+    cluster_wait(S);  // all CTAs run: their shared memory may be written
+    for (int i = tid; i < S * G; i += kThreads) {
+      const int r = i / G, h = i - r * G;
+      const float2 ml = cta_ml(h);
+      float* dst = const_cast<float*>(cluster_peer(s_recv_ml, r)) + (rank * GP + h) * 2;
+      dst[0] = ml.x;
+      dst[1] = ml.y;
+    }
+    for (int i = tid; i < G * HD; i += kThreads) {
+      const int r = i / share;
+      const_cast<float*>(cluster_peer(s_recv, r))[rank * share + i - r * share] =
+          cta_o(i, cta_ml(i / HD).x);
+    }
+    cluster_barrier(S);
+    auto ml_of = [&](int x, int h) { return s_recv_ml + (x * GP + h) * 2; };
+    const int i0 = rank * share;
+    for (int i = tid; i < min(share, G * HD - i0); i += kThreads)
+      joined_o(i0 + i, [&](int x) { return s_recv + x * share + i; }, ml_of);
+    if (WEIGHTS) norm_of(ml_of);
+  } else {
+    for (int i = tid; i < GP * HD; i += kThreads) s_o[i] = cta_o(i, cta_ml(i / HD).x);
+    if (tid < GP) {
+      const float2 ml = cta_ml(tid);
+      s_ml[tid * 2] = ml.x;
+      s_ml[tid * 2 + 1] = ml.y;
+    }
+    cluster_barrier(S);
+    auto ml_of = [&](int x, int h) {
+      return S == 1 ? &s_ml[h * 2] : cluster_peer(&s_ml[h * 2], x);
+    };
+    for (int i = rank * kThreads + tid; i < G * HD; i += S * kThreads)
+      joined_o(i, [&](int x) { return S == 1 ? &s_o[i] : cluster_peer(&s_o[i], x); }, ml_of);
+    if (WEIGHTS) norm_of(ml_of);
+    if (S > 1) cluster_barrier(S);  // no CTA leaves while another reads its shared memory
+  }
   if constexpr (WEIGHTS) {
     // this CTA's own rows, in the order their units were dealt
     float* wrow = wts + (int64_t)g * p.weight_stride;
@@ -830,7 +875,6 @@ int launch_shape(AttendParams& p, int64_t items, int S, cudaStream_t stream, std
   static std::atomic<uint64_t> attr_done{0};
   using C = Cta<T, HD, WIDE>;
   static_assert(C::kRing >= (C::kWarps * (HD + 2) + HD) * GP * 4, "the outputs reuse the rings");
-  static_assert(C::kRing >= 16 * (HD * 2 + 16) + 32, "q is split in the rings");
   if (items * S > INT32_MAX) {
     *err = "batch * n_kv_heads too large";
     return GLA_ERR_NOT_SUPPORTED;

@@ -141,13 +141,13 @@ class GlaError(RuntimeError):
 
 
 def _ptr(x) -> int | None:
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or x.__class__ is int:
         return x
     dp = getattr(x, "data_ptr", None)
     if dp is not None:
-        return int(dp())
+        return dp()
+    if isinstance(x, int):
+        return x
     raise TypeError(f"expected a device tensor or an address, got {type(x)!r}")
 
 
