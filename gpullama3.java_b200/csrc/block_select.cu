@@ -220,16 +220,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   for (int i = 0; i < kQ; ++i)
     if (i * kThreads + tid < GP * HD) s_q[i * kThreads + tid] = qr[i];
   __syncthreads();
-  float co[kCpl * kPer][GP];
+  // (products of two heads at once: packed FMAs)
+  constexpr int kPairs = GP >= 2 ? GP / 2 : 1;
+  uint64_t co[kCpl * kPer][kPairs];
 #pragma unroll
   for (int c = 0; c < kCpl; ++c) {
     const int el = (sl + c * kLanes) * kPer;  // [0, HD) lo, [HD, 2 HD) hi
     const int d = el < HD ? el : el - HD;
 #pragma unroll
-    for (int h = 0; h < GP; ++h)
+    for (int h = 0; h < kPairs; ++h)
 #pragma unroll
-      for (int p = 0; p < kPer; ++p)
-        co[c * kPer + p][h] = el < 2 * HD ? coefficient(s_q[h * HD + d + p], el < HD) : 0.f;
+      for (int p = 0; p < kPer; ++p) {
+        auto of = [&](int head) {
+          return el < 2 * HD && head < GP ? coefficient(s_q[head * HD + d + p], el < HD) : 0.f;
+        };
+        co[c * kPer + p][h] = pk2(of(2 * h), of(2 * h + 1));
+      }
   }
 
   // keys, M and the keys' range go to rank 0's shared memory
@@ -248,8 +254,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       float acc[kVals];
 #pragma unroll
       for (int i = 0; i < kBlk; ++i) {
+        uint64_t sum[kPairs];
 #pragma unroll
-        for (int h = 0; h < GP; ++h) acc[i * GP + h] = 0.f;
+        for (int h = 0; h < kPairs; ++h) sum[h] = 0;
 #pragma unroll
         for (int c = 0; c < kCpl; ++c) {
           const int chunk = sl + c * kLanes;
@@ -262,10 +269,17 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int p = 0; p < kPer; ++p) {
             const float y = (float)reinterpret_cast<const T*>(&x)[p];
             big = fmaxf(big, fabsf(y));
+            const uint64_t yy = pk2(y, y);
 #pragma unroll
-            for (int h = 0; h < GP; ++h)
-              acc[i * GP + h] = fmaf(co[c * kPer + p][h], y, acc[i * GP + h]);
+            for (int h = 0; h < kPairs; ++h) sum[h] = fma2(co[c * kPer + p][h], yy, sum[h]);
           }
+        }
+#pragma unroll
+        for (int h = 0; h < kPairs; ++h) {
+          float a, b2;
+          upk2(sum[h], a, b2);
+          acc[i * GP + 2 * h] = a;
+          if (GP > 1) acc[i * GP + (2 * h + 1) % GP] = b2;
         }
       }
       __syncwarp();  // read out by every lane
@@ -298,7 +312,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   for (int h = 0; h < GP; ++h) {
     float cs = 0.f;
 #pragma unroll
-    for (int e = 0; e < kCpl * kPer; ++e) cs += fabsf(co[e][h]);
+    for (int e = 0; e < kCpl * kPer; ++e) {
+      float a, b2;
+      upk2(co[e][h / 2], a, b2);
+      cs += fabsf(h % 2 ? b2 : a);
+    }
     cs = cs == 0.f ? 0.f : cs * big;  // an infinite bound that no coefficient meets
 #pragma unroll
     for (int m = kLanes / 2; m > 0; m >>= 1) cs += __shfl_xor_sync(0xffffffffu, cs, m);
@@ -437,10 +455,10 @@ int launch_select(const SelectRequest& r, const DeviceInfo& dev, cudaStream_t st
     *err = "too many blocks for one selection: use larger blocks";
     return GLA_ERR_NOT_SUPPORTED;
   }
-  // as many CTAs a (sequence, kv head) as fill the device (two an SM), while each
-  // still has 64 blocks to score
+  // as many CTAs a (sequence, kv head) as the device holds at once (two an SM: a second
+  // wave would start over with its queries' loads), while each still has 64 blocks
   int S = 1;
-  while (S < 16 && items * S < 2 * dev.sms && max_nb > 64 * S) S *= 2;
+  while (S < 16 && items * S <= dev.sms && max_nb > 64 * S) S *= 2;
   if (items * S > INT32_MAX) {
     *err = "batch * n_kv_heads too large";
     return GLA_ERR_NOT_SUPPORTED;

@@ -241,17 +241,25 @@ struct WarpF16 {
   // q of the group's heads, scaled and split into shared memory, then to registers.
   static constexpr int kQBytes = 16 * kPitch + 32;
 
+  // This thread's part of q, loaded ahead of its use: a warp takes every W-th head.
   template <int W>
-  __device__ __forceinline__ void init(const float* q, int G, float scale_log2, char* scratch,
+  struct Query {
+    float x[8 / W][HD / 32];
+    __device__ __forceinline__ void load(const float* q, int G, int warp, int lane) {
+#pragma unroll
+      for (int j = 0; j < 8 / W; ++j)
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i)
+          x[j][i] = warp + j * W < G ? __ldg(q + (warp + j * W) * HD + i * 32 + lane) : 0.f;
+    }
+  };
+
+  template <int W>
+  __device__ __forceinline__ void init(const Query<W>& in, float scale_log2, char* scratch,
                                        int warp, int lane) {
+    const auto& x = in.x;
     __half* s_q = reinterpret_cast<__half*>(scratch);                 // [16][HD + 8]
     float* s_f = reinterpret_cast<float*>(scratch + 16 * kPitch);     // [8]
-    float x[8 / W][HD / 32];
-#pragma unroll
-    for (int j = 0; j < 8 / W; ++j)  // one head a warp at a time
-#pragma unroll
-      for (int i = 0; i < HD / 32; ++i)
-        x[j][i] = warp + j * W < G ? q[(int64_t)(warp + j * W) * HD + i * 32 + lane] : 0.f;
 #pragma unroll
     for (int j = 0; j < 8 / W; ++j) {
       const int h = warp + j * W;
@@ -391,22 +399,36 @@ struct WarpF32 {
 
   static constexpr int kQBytes = HD / 8 * 32 * 16;
 
+  // This thread's part of q, loaded ahead of its use.  The fragment of step ks is
+  // (hi, lo) of channels 8 ks + (lane & 3) and + 4 of head lane / 4; a warp takes
+  // every W-th step.
   template <int W>
-  __device__ __forceinline__ void init(const float* q, int G, float scale_log2, char* scratch,
+  struct Query {
+    static constexpr int kSteps = (HD / 8 + W - 1) / W;
+    float x[kSteps], y[kSteps];
+    __device__ __forceinline__ void load(const float* q, int G, int warp, int lane) {
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        const int h = lane >> 2, ch = (warp + j * W) * 8 + (lane & 3);
+        const bool in = h < G && ch < HD;
+        x[j] = in ? __ldg(q + h * HD + ch) : 0.f;
+        y[j] = in ? __ldg(q + h * HD + ch + 4) : 0.f;
+      }
+    }
+  };
+
+  template <int W>
+  __device__ __forceinline__ void init(const Query<W>& in, float scale_log2, char* scratch,
                                        int warp, int lane) {
     uint4* s_q = reinterpret_cast<uint4*>(scratch);
-    // fragment of step ks: (hi, lo) of channels 8 ks + (lane & 3) and + 4 of head lane / 4
-    for (int i = warp * 32 + lane; i < HD / 8 * 32; i += W * 32) {
-      const int l = i & 31, h = l >> 2, ch = (i >> 5) * 8 + (l & 3);
-      float x = 0.f, y = 0.f;
-      if (h < G) {
-        x = q[(int64_t)h * HD + ch];
-        y = q[(int64_t)h * HD + ch + 4];
+#pragma unroll
+    for (int j = 0; j < Query<W>::kSteps; ++j) {
+      if (warp + j * W < HD / 8) {
+        uint4 f;
+        split_tf32(in.x[j], f.x, f.y);
+        split_tf32(in.y[j], f.z, f.w);
+        s_q[(warp + j * W) * 32 + lane] = f;
       }
-      uint4 f;
-      split_tf32(x, f.x, f.y);
-      split_tf32(y, f.z, f.w);
-      s_q[i] = f;
     }
     __syncthreads();
     factor = scale_log2;
@@ -555,6 +577,7 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   __shared__ float s_recv[WIDE ? GP * HD + 16 : 1];
   __shared__ float s_recv_ml[WIDE ? 16 * GP * 2 : 1];
   __shared__ float s_norm[GP * 2];
+  __shared__ float s_wt[kWarps][GP];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int S = p.S;
   const int rank = S > 1 ? (int)(blockIdx.x % (unsigned)S) : 0;
@@ -566,6 +589,17 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   // first free places of this kernel's SMs and crowd there (109 us against 73 for
   // 131,072 rows).
   if (!p.part) pdl_launch_dependents();
+  // q, the first units' ids, the length and the pointers are loaded side by side
+  typename Warp::template Query<kWarps> query;
+  query.load(p.q + ((int64_t)b * p.n_heads + (int64_t)g * G) * HD, G, warp, lane);
+  const int32_t* ids = BLOCKS ? p.block_ids + (int64_t)item * p.n_sel : nullptr;
+  const int32_t listed = BLOCKS ? p.n_sel << (p.br_shift - kShift) : 0;
+  auto id_of = [&](int32_t u) {
+    return BLOCKS && u < listed ? __ldg(ids + (u >> (p.br_shift - kShift))) : -1;
+  };
+  int32_t id[kStages + 1];
+#pragma unroll
+  for (int s = 0; s <= kStages; ++s) id[s] = id_of((rank + s * S) * kWarps + warp);
   int32_t n = clamped_rows(p.n_pos, b, p.max_n_pos, p.status);
   if (WEIGHTS && p.part && (int64_t)rank * p.part_rows >= n) return;
   const T* k = static_cast<const T*>(p.k_ptrs[b]);
@@ -575,10 +609,8 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   if (WEIGHTS && !usable_weights(wts, p.status)) n = 0;
   k += (int64_t)g * HD;
   v += (int64_t)g * HD;
-  const int32_t* ids = BLOCKS ? p.block_ids + (int64_t)item * p.n_sel : nullptr;
   // units of this CTA's warps: a cluster's deal, or this part's
-  int32_t units = BLOCKS ? (n > 0 ? p.n_sel << (p.br_shift - kShift) : 0)
-                         : (int32_t)(((int64_t)n + U - 1) / U);
+  int32_t units = BLOCKS ? (n > 0 ? listed : 0) : (int32_t)(((int64_t)n + U - 1) / U);
   int32_t cta_first = rank * kWarps, stride = S * kWarps;
   if (WEIGHTS && p.part) {
     cta_first = rank * (p.part_rows / U);
@@ -596,10 +628,6 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   // ring's other units are under way too.
   const int32_t mine = units > first ? (units - first - 1) / stride + 1 : 0;
   int32_t row_of[kStages];
-  // ids are loaded a step before the rows they name
-  auto id_of = [&](int32_t i) {
-    return BLOCKS && i < mine ? __ldg(ids + ((first + i * stride) >> (p.br_shift - kShift))) : -1;
-  };
   auto fetch = [&](int s, int32_t i, int32_t id) {
     row_of[s] = -1;
     if (i < mine) {
@@ -609,16 +637,12 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
     }
     cp_async_commit();
   };
-  int32_t id[kStages + 1];
-#pragma unroll
-  for (int s = 0; s <= kStages; ++s) id[s] = id_of(s);
 #pragma unroll
   for (int s = 0; s < kStages; ++s) fetch(s, s, id[s]);
-  int32_t next_id = id[kStages];
+  int32_t next_id = id[kStages];  // ids are loaded a step before the rows they name
   if (WIDE) cluster_arrive(S);
   Warp w;  // while the first units are under way
-  w.template init<kWarps>(p.q + ((int64_t)b * p.n_heads + (int64_t)g * G) * HD, G, p.scale_log2,
-                          s_q, warp, lane);
+  w.template init<kWarps>(query, p.scale_log2, s_q, warp, lane);
   for (int32_t i0 = 0; i0 < mine; i0 += kStages) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) {
@@ -630,7 +654,7 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
                                    p.score_pitch, G, s_q, lane);
         __syncwarp();  // and read out by every lane
         fetch(s, i0 + s + kStages, next_id);
-        next_id = id_of(i0 + s + kStages + 1);
+        next_id = id_of(first + (i0 + s + kStages + 1) * stride);
       }
     }
   }
@@ -644,22 +668,28 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   float* s_o = sml + kWarps * GP * 2;
   w.store(so + warp * GP * HD, sml + warp * GP * 2, lane);
   __syncthreads();
-  auto cta_ml = [&](int h) {
-    float top = -INFINITY, sum = 0.f;
+  // each head's largest m, its sum, and the warps' weights relative to it
+  if (tid < GP * kWarps) {
+    const int x = tid / GP, h = tid % GP;
+    float top = -INFINITY;
 #pragma unroll
-    for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sml[(x * GP + h) * 2]);
+    for (int y = 0; y < kWarps; ++y) top = fmaxf(top, sml[(y * GP + h) * 2]);
     const float ref = top == -INFINITY ? 0.f : top;
+    s_wt[x][h] = exp2_approx(sml[(x * GP + h) * 2] - ref);
+    if (x == 0) {
+      float sum = 0.f;
 #pragma unroll
-    for (int x = 0; x < kWarps; ++x)
-      sum = fmaf(sml[(x * GP + h) * 2 + 1], exp2_approx(sml[(x * GP + h) * 2] - ref), sum);
-    return make_float2(top, sum);
-  };
-  auto cta_o = [&](int i, float top) {
-    const float ref = top == -INFINITY ? 0.f : top;
+      for (int y = 0; y < kWarps; ++y)
+        sum = fmaf(sml[(y * GP + h) * 2 + 1], exp2_approx(sml[(y * GP + h) * 2] - ref), sum);
+      s_ml[h * 2] = top;
+      s_ml[h * 2 + 1] = sum;
+    }
+  }
+  __syncthreads();
+  auto cta_o = [&](int i) {
     float acc = 0.f;
 #pragma unroll
-    for (int x = 0; x < kWarps; ++x)
-      acc = fmaf(so[x * GP * HD + i], exp2_approx(sml[(x * GP + i / HD) * 2] - ref), acc);
+    for (int x = 0; x < kWarps; ++x) acc = fmaf(so[x * GP * HD + i], s_wt[x][i / HD], acc);
     return acc;
   };
   // the outputs of a list of (o, m, l): o_of(x) and ml_of(x, h) of rank x
@@ -692,8 +722,9 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   };
   if (WEIGHTS && p.part) {  // joined by attend_join_kernel
     float* part = p.part + ((int64_t)item * S + rank) * G * HD;
-    for (int i = tid; i < G * HD; i += kThreads) part[i] = cta_o(i, cta_ml(i / HD).x);
-    if (tid < G) p.part_ml[((int64_t)item * G + tid) * S + rank] = cta_ml(tid);
+    for (int i = tid; i < G * HD; i += kThreads) part[i] = cta_o(i);
+    if (tid < G)
+      p.part_ml[((int64_t)item * G + tid) * S + rank] = make_float2(s_ml[tid * 2], s_ml[tid * 2 + 1]);
     return;
   }
   if (WIDE && S > 1) {
@@ -702,15 +733,13 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
     cluster_wait(S);  // all CTAs run: their shared memory may be written
     for (int i = tid; i < S * G; i += kThreads) {
       const int r = i / G, h = i - r * G;
-      const float2 ml = cta_ml(h);
       float* dst = const_cast<float*>(cluster_peer(s_recv_ml, r)) + (rank * GP + h) * 2;
-      dst[0] = ml.x;
-      dst[1] = ml.y;
+      dst[0] = s_ml[h * 2];
+      dst[1] = s_ml[h * 2 + 1];
     }
     for (int i = tid; i < G * HD; i += kThreads) {
       const int r = i / share;
-      const_cast<float*>(cluster_peer(s_recv, r))[rank * share + i - r * share] =
-          cta_o(i, cta_ml(i / HD).x);
+      const_cast<float*>(cluster_peer(s_recv, r))[rank * share + i - r * share] = cta_o(i);
     }
     cluster_barrier(S);
     auto ml_of = [&](int x, int h) { return s_recv_ml + (x * GP + h) * 2; };
@@ -719,12 +748,7 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
       joined_o(i0 + i, [&](int x) { return s_recv + x * share + i; }, ml_of);
     if (WEIGHTS) norm_of(ml_of);
   } else {
-    for (int i = tid; i < GP * HD; i += kThreads) s_o[i] = cta_o(i, cta_ml(i / HD).x);
-    if (tid < GP) {
-      const float2 ml = cta_ml(tid);
-      s_ml[tid * 2] = ml.x;
-      s_ml[tid * 2 + 1] = ml.y;
-    }
+    for (int i = tid; i < GP * HD; i += kThreads) s_o[i] = cta_o(i);
     cluster_barrier(S);
     auto ml_of = [&](int x, int h) {
       return S == 1 ? &s_ml[h * 2] : cluster_peer(&s_ml[h * 2], x);
@@ -932,13 +956,20 @@ int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t strea
                              (int32_t)shares);
     }
   }
-  // CTAs of a cluster: as many as fill the device, while every warp still has a
-  // unit; wide ones if 16 slim ones an item would not fill it
-  const bool wide = items * 16 < 3 * dev.sms;
-  const int warps = wide ? 8 : 4;
-  const int64_t slots = wide ? dev.sms : 3 * dev.sms;
-  int S = 1;
-  while (S < 16 && items * S < slots && units > (int64_t)warps * S) S *= 2;
+  // CTAs of a cluster: as many as the device holds at once, while every warp still
+  // has a unit; wide or slim ones, whichever makes more warps (wide ones hold 8
+  // clusters of 16, one a GPC)
+  auto cluster_of = [&](bool w) {
+    const int64_t slots = w ? dev.sms : 3 * dev.sms;
+    int S = 1;
+    while (S < 16 && items * S * 2 <= slots && units > (int64_t)(w ? 8 : 4) * S &&
+           !(w && S == 8 && items > 8))
+      S *= 2;
+    return S;
+  };
+  const int sw = cluster_of(true), ss = cluster_of(false);
+  const bool wide = items * sw <= dev.sms && sw * 8 >= ss * 4;
+  const int S = wide ? sw : ss;
   return wide ? launch_shape<T, HD, BLOCKS, true>(p, items, S, stream, err)
               : launch_shape<T, HD, BLOCKS, false>(p, items, S, stream, err);
 }
