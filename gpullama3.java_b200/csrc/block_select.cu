@@ -102,7 +102,7 @@ struct Shape {
 
 // The ring and the 64-bit keys' upper words share their bytes.
 template <class T, int HD, int GP>
-size_t select_smem(int64_t max_nb) {
+size_t select_smem(int64_t max_nb) {  // max_nb: a multiple of 4
   using Sh = Shape<T, HD, GP>;
   return (size_t)std::max<int64_t>(Sh::kRing, max_nb * 4) + (size_t)max_nb * 4;
 }
@@ -335,6 +335,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     max0[rank * kWarps + warp] = kmax;
   }
   if (tid == 0) s_near_n = s_sure_n = 0;
+  if (rank == 0) fill_up_keys(s_lower, nc);
   cluster_barrier(S);
   if (rank != 0) return;
 
@@ -342,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   for (int i = tid; i < n_first + n_last; i += kThreads)
     ids[i < n_first ? i : pick + i] = i < n_first ? i : nc + i;
   ids += n_first;
-  auto key_of = [&](int32_t i) { return s_lower[i]; };
+  const SharedKeys key_of{s_lower};
   auto emit = [&](int32_t i, uint32_t at) { ids[at] = n_first + i; };
   mag = 0.f;
   kmin = ~0u;
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   }
   __syncthreads();
-  auto slot_of = [&](int32_t i) { return (uint64_t)s_upper[i] << 32 | s_lower[i]; };
+  auto slot_of = keys_by([&](int32_t i) { return (uint64_t)s_upper[i] << 32 | s_lower[i]; });
   const Threshold<uint64_t> th64 = find_threshold<kThreads, uint64_t>(
       sh, 1, nc, (uint32_t)pick, (uint64_t)0, ~(uint64_t)0, slot_of);
   emit_chosen<kThreads, uint64_t>(sh, 1, 0, nc, th64, slot_of, emit);
@@ -450,7 +451,7 @@ int launch_select(const SelectRequest& r, const DeviceInfo& dev, cudaStream_t st
   int32_t br_shift = 0;
   while ((1 << br_shift) < r.block_rows) ++br_shift;
   const int64_t items = (int64_t)r.batch * r.n_kv;
-  const int64_t max_nb = ((int64_t)r.max_n_pos + r.block_rows - 1) / r.block_rows;
+  const int64_t max_nb = (((int64_t)r.max_n_pos + r.block_rows - 1) / r.block_rows + 3) / 4 * 4;
   if (max_nb > kMaxSelectBlocks) {
     *err = "too many blocks for one selection: use larger blocks";
     return GLA_ERR_NOT_SUPPORTED;

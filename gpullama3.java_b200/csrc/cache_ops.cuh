@@ -146,7 +146,8 @@ __device__ __forceinline__ float key_score(uint32_t key) {
 // The k largest of the keys that the CTAs of a cluster hold together, ties to
 // the lowest index.  CTA r holds the n_local keys key(0..n_local-1) of a
 // contiguous index range, ranges ascending with the rank; 0 < k < all keys.
-// The keys are walked once a pass: they belong in shared memory.
+// The keys are walked once a pass, and the walks are bound by instructions: 32-bit
+// keys in shared memory (SharedKeys) are taken four at a time.
 //
 // find_threshold: radix selection, 8 bits a pass over the range [kmin, kmax] of the
 // keys (key_range finds it: full-width digits would put nearly all scores into a few
@@ -160,7 +161,33 @@ __device__ __forceinline__ float key_score(uint32_t key) {
 // chosen indices, so the list ascends with no barrier inside:
 // emit(local index, position in the list of all chosen).
 // ---------------------------------------------------------------------------
-constexpr int kSelectWarps = 16;  // at most
+// 32-bit keys in shared memory, 16-byte aligned and filled up with keys of 0 to a
+// multiple of 4.  (A filling key ranks behind every real one: 0 is the lowest and it
+// has the highest index of its CTA; walks that break ties by index leave it out.)
+struct SharedKeys {
+  static constexpr bool kQuads = true;
+  const uint32_t* p;
+  __device__ __forceinline__ uint32_t operator()(int32_t i) const { return p[i]; }
+  __device__ __forceinline__ uint4 quad(int32_t q) const {
+    return reinterpret_cast<const uint4*>(p)[q];
+  }
+};
+__device__ __forceinline__ void fill_up_keys(uint32_t* p, int32_t n) {
+  if (threadIdx.x < 4 && (n & 3) + (int)threadIdx.x < 4 && (n & 3)) p[n + threadIdx.x] = 0;
+}
+// Any other keys: one at a time.
+template <class F>
+struct KeysBy {
+  static constexpr bool kQuads = false;
+  F f;
+  __device__ __forceinline__ auto operator()(int32_t i) const { return f(i); }
+};
+template <class F>
+__device__ __forceinline__ KeysBy<F> keys_by(F f) {
+  return KeysBy<F>{f};
+}
+
+constexpr int kSelectWarps = 32;  // at most
 struct SelectScratch {
   uint32_t hist[2][256];
   uint32_t warp_sum[8];
@@ -221,11 +248,23 @@ __device__ __forceinline__ Threshold<Key> find_threshold(SelectScratch& sh, int 
   Key base = kmin, span = kmax - kmin;  // the range is [base, base + span]
   int shift = bit_count(span) > 8 ? bit_count(span) - 8 : 0;
   for (;; buf ^= 1) {
+    // (a key below base wraps to a distance beyond span)
+    auto count = [&](Key kv) {
+      const Key d = kv - base;
+      if (d <= span) atomicAdd(&sh.hist[buf][(uint32_t)(d >> shift)], 1u);
+    };
+    if constexpr (KeyFn::kQuads) {
+#pragma unroll 2
+      for (int32_t q = tid; q < (n_local + 3) / 4; q += THREADS) {
+        const uint4 kv = key.quad(q);
+        count(kv.x);
+        count(kv.y);
+        count(kv.z);
+        count(kv.w);
+      }
+    } else {
 #pragma unroll 4
-    for (int32_t i = tid; i < n_local; i += THREADS) {
-      const Key kv = key(i);
-      if (kv >= base && kv - base <= span)
-        atomicAdd(&sh.hist[buf][(uint32_t)((kv - base) >> shift) & 255u], 1u);
+      for (int32_t i = tid; i < n_local; i += THREADS) count(key(i));
     }
     cluster_barrier(S);
     uint32_t mine = 0;
@@ -274,15 +313,28 @@ __device__ __forceinline__ void emit_chosen(SelectScratch& sh, int S, int rank, 
   static_assert(W <= kSelectWarps, "per-warp counts");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t need = th.need;
-  // this warp's share of the CTA's keys: whole warps of them, contiguous
-  const int32_t share = ((n_local + THREADS - 1) / THREADS) * 32;
+  // this warp's share of the CTA's keys: whole warps of (four) keys, contiguous
+  constexpr int kStep = KeyFn::kQuads ? 128 : 32;
+  const int32_t share = ((n_local + W * kStep - 1) / (W * kStep)) * kStep;
   const int32_t w_lo = min(warp * share, n_local), w_hi = min(w_lo + share, n_local);
+  const bool fast = KeyFn::kQuads && th.whole;
   uint32_t above = 0, at = 0;
+  if constexpr (KeyFn::kQuads) {
+    if (fast) {
 #pragma unroll 4
-  for (int32_t i = w_lo + lane; i < w_hi; i += 32) {
-    const Key kv = key(i);
-    above += th.above(kv);
-    at += th.at(kv);
+      for (int32_t q = w_lo / 4 + lane; q < (w_hi + 3) / 4; q += 32) {
+        const uint4 kv = key.quad(q);
+        above += (kv.x >= th.lo) + (kv.y >= th.lo) + (kv.z >= th.lo) + (kv.w >= th.lo);
+      }
+    }
+  }
+  if (!fast) {
+#pragma unroll 4
+    for (int32_t i = w_lo + lane; i < w_hi; i += 32) {
+      const Key kv = key(i);
+      above += th.above(kv);
+      at += th.at(kv);
+    }
   }
   above = __reduce_add_sync(0xffffffffu, above);
   at = __reduce_add_sync(0xffffffffu, at);
@@ -315,16 +367,29 @@ __device__ __forceinline__ void emit_chosen(SelectScratch& sh, int S, int rank, 
   at_before = __reduce_add_sync(0xffffffffu, at_before);
   uint32_t out = before + (at_before < need ? at_before : need);
   const unsigned below = (1u << lane) - 1;
-  if (th.whole) {
-#pragma unroll 4
-    for (int32_t i0 = w_lo; i0 < w_hi; i0 += 32) {
-      const int32_t i = i0 + lane;
-      const bool take = i < w_hi && key(min(i, w_hi - 1)) >= th.lo;
-      const unsigned bt = __ballot_sync(0xffffffffu, take);
-      if (take) emit(i, out + __popc(bt & below));
-      out += __popc(bt);
+  if constexpr (KeyFn::kQuads) {
+    if (fast) {
+#pragma unroll 2
+      for (int32_t i0 = w_lo; i0 < w_hi; i0 += 128) {
+        const int32_t i = i0 + lane * 4;
+        uint4 kv = make_uint4(0, 0, 0, 0);
+        if (i < w_hi) kv = key.quad(i / 4);
+        const bool a = kv.x >= th.lo, b = kv.y >= th.lo, c = kv.z >= th.lo, d = kv.w >= th.lo;
+        // prefix sums of the lanes' counts, 0 to 4, by their binary digits
+        const uint32_t mine = (uint32_t)a + b + c + d;
+        const unsigned b0 = __ballot_sync(0xffffffffu, mine & 1);
+        const unsigned b1 = __ballot_sync(0xffffffffu, mine & 2);
+        const unsigned b2 = __ballot_sync(0xffffffffu, mine & 4);
+        uint32_t pos = out + __popc(b0 & below) + 2 * __popc(b1 & below) + 4 * __popc(b2 & below);
+        if (a) emit(i, pos++);
+        if (b) emit(i + 1, pos++);
+        if (c) emit(i + 2, pos++);
+        if (d) emit(i + 3, pos);
+        out += __popc(b0) + 2 * __popc(b1) + 4 * __popc(b2);
+      }
     }
-  } else {
+  }
+  if (!fast) {
     for (int32_t i0 = w_lo; i0 < w_hi; i0 += 32) {
       const int32_t i = i0 + lane;
       const bool in = i < w_hi;

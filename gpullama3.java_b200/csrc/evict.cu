@@ -18,7 +18,7 @@ namespace gla {
 
 namespace {
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kMoveThreads = 256;
 
 __global__ void __launch_bounds__(kSelThreads)
@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(kSelThreads)
                         const int32_t* __restrict__ n_pos, int32_t max_n_pos, int32_t n_keep,
                         int32_t n_recent, int32_t* __restrict__ kept, int32_t n_kv, int S,
                         int32_t key_cap, int32_t* __restrict__ status) {
-  extern __shared__ uint32_t s_key[];
+  extern __shared__ __align__(16) uint32_t s_key[];
   __shared__ SelectScratch sh;
   pdl_wait();
   pdl_launch_dependents();
@@ -52,13 +52,14 @@ __global__ void __launch_bounds__(kSelThreads)
   const float* mine = w + (int64_t)g * weight_stride + lo;
   const bool fits = (older + S - 1) / S <= key_cap;  // (not so past 16 CTAs' shared memory)
   uint32_t kmin = ~0u, kmax = 0;
-#pragma unroll 4
+#pragma unroll 8
   for (int32_t i = tid; i < hi - lo; i += kSelThreads) {
     const uint32_t k = order_key(__ldcg(mine + i));
     if (fits) s_key[i] = k;
     kmin = min(kmin, k);
     kmax = max(kmax, k);
   }
+  if (fits) fill_up_keys(s_key, hi - lo);
   key_range<kSelThreads>(sh, S, &kmin, &kmax);  // (a barrier: the keys are staged)
   auto select = [&](auto key) {
     const Threshold<uint32_t> th = find_threshold<kSelThreads, uint32_t>(
@@ -68,9 +69,9 @@ __global__ void __launch_bounds__(kSelThreads)
   };
   // the ranks' shares differ by rounding alone, and every rank takes the same way
   if (fits)
-    select([&](int32_t i) { return s_key[i]; });
+    select(SharedKeys{s_key});
   else
-    select([&](int32_t i) { return order_key(__ldcg(mine + i)); });
+    select(keys_by([&](int32_t i) { return order_key(__ldcg(mine + i)); }));
 }
 
 // Kept rows of one kv head to another cache: thread = (row, 16-byte chunk).
@@ -281,14 +282,13 @@ int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stre
                  std::string* err) {
   static std::atomic<uint64_t> attr_done{0};
   const int64_t items = (int64_t)r.batch * r.n_kv;
-  // a CTA for every 8192 weights (a cluster's barriers cost about as much as walking
-  // that many), as long as that does not exceed four CTAs an SM; and enough for the
-  // keys to fit shared memory (past 16 CTAs the rest is read again a pass)
-  const int64_t most_keys = (dev.smem_optin - 8 * 1024) / 4;
+  // One CTA a kv head up to 32,768 weights: each of the passes of a cluster costs it
+  // about 1.5 us in barriers and remote counts, more than walking that many keys in
+  // shared memory (16 sequences of up to 32,768 rows: 28 us with clusters of 4).
+  // Past 16 CTAs' shared memory the weights are read again a pass.
+  const int64_t most_keys = (dev.smem_optin - 12 * 1024) / 4;
   int S = 1;
-  while (S < 16 && ((items * S < 3 * dev.sms && r.max_n_pos > (int64_t)8192 * S) ||
-                    r.max_n_pos > most_keys * S))
-    S *= 2;
+  while (S < 16 && r.max_n_pos > (int64_t)32768 * S) S *= 2;
   const int32_t key_cap =
       (int32_t)std::min<int64_t>(most_keys, ((int64_t)r.max_n_pos + S - 1) / S);
   if (items * S > INT32_MAX) {
@@ -296,7 +296,7 @@ int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stre
     return GLA_ERR_NOT_SUPPORTED;
   }
   int rc = launch_clusters(evict_select_kernel, (unsigned)(items * S), kSelThreads,
-                           (size_t)key_cap * 4, S, attr_done,
+                           ((size_t)key_cap + 3) / 4 * 16, S, attr_done,
                            stream, "evict selection", err,
                            (const float* const*)r.weight_ptrs, r.weight_stride, r.n_pos,
                            r.max_n_pos, r.n_keep, r.n_recent, r.kept, r.n_kv, S, key_cap, r.status);
