@@ -447,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 template <class T, int HD, int GP>
 int launch_select(const SelectRequest& r, const DeviceInfo& dev, cudaStream_t stream,
                   std::string* err) {
-  static std::atomic<uint64_t> attr_done{0};
+  static ClusterKernel ck;
   int32_t br_shift = 0;
   while ((1 << br_shift) < r.block_rows) ++br_shift;
   const int64_t items = (int64_t)r.batch * r.n_kv;
@@ -456,16 +456,20 @@ int launch_select(const SelectRequest& r, const DeviceInfo& dev, cudaStream_t st
     *err = "too many blocks for one selection: use larger blocks";
     return GLA_ERR_NOT_SUPPORTED;
   }
-  // as many CTAs a (sequence, kv head) as the device holds at once (two an SM: a second
-  // wave would start over with its queries' loads), while each still has 64 blocks
+  // as many CTAs a (sequence, kv head) as the device holds at once (a second wave would
+  // start over with its queries' loads), while each still has 64 blocks
+  const size_t smem = select_smem<T, HD, GP>(max_nb);
   int S = 1;
-  while (S < 16 && items * S <= dev.sms && max_nb > 64 * S) S *= 2;
+  while (S < 16 && max_nb > 64 * S && items * S * 2 <= 2 * dev.sms &&
+         items <= clusters_held(block_select_kernel<T, HD, GP>, ck, kThreads,
+                                select_smem<T, HD, GP>(4), 2 * S, dev))
+    S *= 2;
   if (items * S > INT32_MAX) {
     *err = "batch * n_kv_heads too large";
     return GLA_ERR_NOT_SUPPORTED;
   }
   return launch_clusters(block_select_kernel<T, HD, GP>, (unsigned)(items * S), kThreads,
-                         select_smem<T, HD, GP>(max_nb), S, attr_done, stream, "block selection", err, r.q,
+                         smem, S, ck, stream, "block selection", err, r.q,
                          reinterpret_cast<const T* const*>(r.bounds_ptrs), r.n_pos, r.max_n_pos,
                          r.block_ids, r.n_heads, r.n_kv, br_shift, r.n_sel, r.n_first, r.n_last, S,
                          (int32_t)max_nb, r.status);

@@ -7,6 +7,7 @@
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <string>
 
 #include "gla_common.cuh"
@@ -73,47 +74,91 @@ __device__ __forceinline__ const T* cluster_peer(const T* p, int rank) {
   return reinterpret_cast<const T*>(out);
 }
 
-// Launches `kern` in clusters of S CTAs (grid a multiple of S) behind the
-// preceding kernel of the stream (programmatic dependent launch: the kernel
-// itself waits for it).  Clusters above 8 CTAs need the opt-in attribute.
-template <class... Params, class... Args>
-int launch_clusters(void (*kern)(Params...), unsigned grid, int threads, size_t smem, int S,
-                    std::atomic<uint64_t>& attr_done, cudaStream_t stream, const char* what,
-                    std::string* err, Args... args) {
+// What a kernel's cluster launches need once a device: raised limits (shared
+// memory, clusters above 8 CTAs), and how many clusters of 1, 2, 4, 8 and 16 CTAs
+// the device holds at once (a cluster lies in one GPC, so fewer than its SMs
+// suggest: 7 of 16 CTAs at one CTA an SM of 148).
+struct ClusterKernel {
+  std::atomic<uint64_t> attr_done{0};  // bit d: device d
+  std::atomic<int> held[5] = {};       // 0: not asked yet (all devices are alike)
+};
+
+template <class... Params>
+int prepare_clusters(void (*kern)(Params...), ClusterKernel& ck, const char* what,
+                     std::string* err) {
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = dev < 64 ? (1ull << dev) : 0;
-  if (!bit || !(attr_done.load(std::memory_order_acquire) & bit)) {
-    int optin = 0;
-    cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
-    cudaFuncAttributes fa;
-    cudaError_t e = cudaFuncGetAttributes(&fa, kern);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               optin - (int)fa.sharedSizeBytes);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      *err = std::string(what) + " attributes: " + cudaGetErrorString(e);
-      return GLA_ERR_CUDA;
-    }
-    if (bit) attr_done.fetch_or(bit, std::memory_order_acq_rel);
+  if (bit && (ck.attr_done.load(std::memory_order_acquire) & bit)) return GLA_OK;
+  int optin = 0;
+  cudaDeviceGetAttribute(&optin, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  cudaFuncAttributes fa;
+  cudaError_t e = cudaFuncGetAttributes(&fa, kern);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             optin - (int)fa.sharedSizeBytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    *err = std::string(what) + " attributes: " + cudaGetErrorString(e);
+    return GLA_ERR_CUDA;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
+  if (bit) ck.attr_done.fetch_or(bit, std::memory_order_acq_rel);
+  return GLA_OK;
+}
+
+inline void cluster_config(cudaLaunchConfig_t* cfg, cudaLaunchAttribute (&attr)[2], unsigned grid,
+                           int threads, size_t smem, int S, cudaStream_t stream) {
+  cfg->gridDim = dim3(grid);
+  cfg->blockDim = dim3((unsigned)threads);
+  cfg->dynamicSmemBytes = smem;
+  cfg->stream = stream;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = (unsigned)S;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = S > 1 ? 2 : 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = S > 1 ? 2 : 1;
+}
+
+// Clusters of S CTAs that the device holds at once (a guess if it cannot say).
+template <class... Params>
+int clusters_held(void (*kern)(Params...), ClusterKernel& ck, int threads, size_t smem, int S,
+                  const DeviceInfo& dev) {
+  int slot = 0;
+  while ((1 << slot) < S) ++slot;
+  int n = ck.held[slot].load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  std::string err;
+  if (prepare_clusters(kern, ck, "cluster", &err) != GLA_OK) return std::max(1, dev.sms / S);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cluster_config(&cfg, attr, (unsigned)S, threads, smem, S, nullptr);
+  cfg.attrs = attr + 1;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = std::max(1, dev.sms / S);
+  }
+  ck.held[slot].store(n, std::memory_order_relaxed);
+  return n;
+}
+
+// Launches `kern` in clusters of S CTAs (grid a multiple of S) behind the
+// preceding kernel of the stream (programmatic dependent launch: the kernel
+// itself waits for it).
+template <class... Params, class... Args>
+int launch_clusters(void (*kern)(Params...), unsigned grid, int threads, size_t smem, int S,
+                    ClusterKernel& ck, cudaStream_t stream, const char* what, std::string* err,
+                    Args... args) {
+  const int rc = prepare_clusters(kern, ck, what, err);
+  if (rc != GLA_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cluster_config(&cfg, attr, grid, threads, smem, S, stream);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) {
     cudaGetLastError();

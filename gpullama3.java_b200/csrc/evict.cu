@@ -280,7 +280,7 @@ int move_dim(const EvictRequest& r, cudaStream_t stream, std::string* err) {
 
 int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stream,
                  std::string* err) {
-  static std::atomic<uint64_t> attr_done{0};
+  static ClusterKernel ck;
   const int64_t items = (int64_t)r.batch * r.n_kv;
   // One CTA a kv head up to 32,768 weights: each of the passes of a cluster costs it
   // about 1.5 us in barriers and remote counts, more than walking that many keys in
@@ -296,7 +296,7 @@ int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stre
     return GLA_ERR_NOT_SUPPORTED;
   }
   int rc = launch_clusters(evict_select_kernel, (unsigned)(items * S), kSelThreads,
-                           ((size_t)key_cap + 3) / 4 * 16, S, attr_done,
+                           ((size_t)key_cap + 3) / 4 * 16, S, ck,
                            stream, "evict selection", err,
                            (const float* const*)r.weight_ptrs, r.weight_stride, r.n_pos,
                            r.max_n_pos, r.n_keep, r.n_recent, r.kept, r.n_kv, S, key_cap, r.status);

@@ -100,7 +100,7 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -108,7 +108,7 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
 }
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint4& a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -581,8 +581,17 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int S = p.S;
   const int rank = S > 1 ? (int)(blockIdx.x % (unsigned)S) : 0;
-  const int item = (int)(blockIdx.x / (unsigned)S);
-  const int b = item / p.n_kv, g = item - b * p.n_kv;
+  int item = (int)(blockIdx.x / (unsigned)S);
+  int b = item / p.n_kv, g = item - b * p.n_kv;
+  if (BLOCKS) {
+    // Kv head by kv head: queries over one cache (a prompt chunk) then find their
+    // head's rows in L2 (256 queries over 32,768 rows of 2 x 2 KB: 211 us against
+    // 252 query by query; separate caches: no difference).
+    const int batch = (int)(gridDim.x / (unsigned)S) / p.n_kv;
+    g = item / batch;
+    b = item - g * batch;
+    item = b * p.n_kv + g;
+  }
   const int G = p.n_heads / p.n_kv;
   pdl_wait();
   // A join that follows is let in only behind the stream: its CTAs would take the
@@ -895,19 +904,36 @@ int32_t part_rows_for(int32_t batch, int32_t n_kv, int64_t max_rows, int unit,
 int64_t score_pitch_for(int64_t max_rows) { return (max_rows + 15) / 16 * 16; }
 
 template <class T, int HD, bool BLOCKS, bool WIDE>
-int launch_shape(AttendParams& p, int64_t items, int S, cudaStream_t stream, std::string* err) {
-  static std::atomic<uint64_t> attr_done{0};
+struct Launch {
   using C = Cta<T, HD, WIDE>;
   static_assert(C::kRing >= (C::kWarps * (HD + 2) + HD) * GP * 4, "the outputs reuse the rings");
-  if (items * S > INT32_MAX) {
-    *err = "batch * n_kv_heads too large";
-    return GLA_ERR_NOT_SUPPORTED;
+
+  static ClusterKernel& state() {
+    static ClusterKernel ck;
+    return ck;
   }
-  p.S = S;
-  return launch_clusters(attend_kernel<T, HD, BLOCKS, WIDE>, (unsigned)(items * S),
-                         C::kThreads, (size_t)C::kRing, p.part ? 1 : S, attr_done, stream,
-                         "attention", err, p);
-}
+  // CTAs of an item's cluster: as many as the device holds at once, while every
+  // warp still has a unit.
+  static int cluster_size(int64_t items, int64_t units, const DeviceInfo& dev) {
+    int S = 1;
+    while (S < 16 && units > (int64_t)C::kWarps * S &&
+           items * S * 2 <= (int64_t)C::kMinCtas * dev.sms &&
+           items <= clusters_held(attend_kernel<T, HD, BLOCKS, WIDE>, state(), C::kThreads,
+                                  (size_t)C::kRing, 2 * S, dev))
+      S *= 2;
+    return S;
+  }
+  // p.part: S parts of an item, else a cluster of S.
+  static int run(AttendParams& p, int64_t items, int S, cudaStream_t stream, std::string* err) {
+    if (items * S > INT32_MAX) {
+      *err = "batch * n_kv_heads too large";
+      return GLA_ERR_NOT_SUPPORTED;
+    }
+    p.S = S;
+    return launch_clusters(attend_kernel<T, HD, BLOCKS, WIDE>, (unsigned)(items * S), C::kThreads,
+                           (size_t)C::kRing, p.part ? 1 : S, state(), stream, "attention", err, p);
+  }
+};
 
 template <class T, int HD, bool BLOCKS>
 int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,
@@ -948,30 +974,21 @@ int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t strea
       const int64_t heads = (int64_t)r.batch * r.n_heads;
       p.part = r.scores + heads * p.score_pitch;
       p.part_ml = reinterpret_cast<float2*>(p.part + heads * parts * r.head_dim);
-      int rc = launch_shape<T, HD, BLOCKS, false>(p, items, (int)parts, stream, err);
+      int rc = Launch<T, HD, BLOCKS, false>::run(p, items, (int)parts, stream, err);
       if (rc != GLA_OK) return rc;
-      static std::atomic<uint64_t> attr_done{0};
+      static ClusterKernel ck;
       return launch_clusters(attend_join_kernel, (unsigned)(items * shares), kJoinThreads, 0, 1,
-                             attr_done, stream, "attention join", err, p, (int32_t)HD, outs,
+                             ck, stream, "attention join", err, p, (int32_t)HD, outs,
                              (int32_t)shares);
     }
   }
-  // CTAs of a cluster: as many as the device holds at once, while every warp still
-  // has a unit; wide or slim ones, whichever makes more warps (wide ones hold 8
-  // clusters of 16, one a GPC)
-  auto cluster_of = [&](bool w) {
-    const int64_t slots = w ? dev.sms : 3 * dev.sms;
-    int S = 1;
-    while (S < 16 && items * S * 2 <= slots && units > (int64_t)(w ? 8 : 4) * S &&
-           !(w && S == 8 && items > 8))
-      S *= 2;
-    return S;
-  };
-  const int sw = cluster_of(true), ss = cluster_of(false);
-  const bool wide = items * sw <= dev.sms && sw * 8 >= ss * 4;
-  const int S = wide ? sw : ss;
-  return wide ? launch_shape<T, HD, BLOCKS, true>(p, items, S, stream, err)
-              : launch_shape<T, HD, BLOCKS, false>(p, items, S, stream, err);
+  // Wide CTAs if they make more warps of an item, or as many without a cluster;
+  // else slim ones, which spread over more SMs (an SM takes in 64 bytes a clock).
+  const int sw = Launch<T, HD, BLOCKS, true>::cluster_size(items, units, dev);
+  const int ss = Launch<T, HD, BLOCKS, false>::cluster_size(items, units, dev);
+  const bool wide = items * sw <= dev.sms && (sw == 1 ? 2 >= ss : 2 * sw > ss);
+  return wide ? Launch<T, HD, BLOCKS, true>::run(p, items, sw, stream, err)
+              : Launch<T, HD, BLOCKS, false>::run(p, items, ss, stream, err);
 }
 
 template <int HD>
