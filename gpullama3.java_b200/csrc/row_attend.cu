@@ -115,10 +115,6 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint4& a, uint32_t
       : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ void lds_f32x2(uint32_t addr, float (&v)[2]) {
-  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(addr));
-}
-
 // x = hi + lo, up to what the matrix instruction drops of lo: hi is x rounded to
 // TF32's 11 bits, so |lo| is at most 2^12 units of x's last place (2^-23 of its
 // power of two), and of its 12 bits 11 count: one unit at most is lost.
@@ -293,8 +289,9 @@ struct WarpF16 {
   }
 
   template <bool WEIGHTS>
-  __device__ __forceinline__ void step(uint32_t slot, int rows, float* scores, int64_t pitch,
+  __device__ __forceinline__ void step(const char* slot_ptr, int rows, float* scores, int64_t pitch,
                                        int G, const char*, int lane) {
+    const uint32_t slot = smem_u32(slot_ptr);
     float s[2][2];
     const int sub = lane >> 3, in = lane & 7;
 #pragma unroll
@@ -441,12 +438,13 @@ struct WarpF32 {
   }
 
   template <bool WEIGHTS>
-  __device__ __forceinline__ void step(uint32_t slot, int rows, float* scores, int64_t pitch,
+  __device__ __forceinline__ void step(const char* slot, int rows, float* scores, int64_t pitch,
                                        int G, const char* scratch, int lane) {
     const uint4* s_q = reinterpret_cast<const uint4*>(scratch);
     // scores: accumulators of 32 channels each, added in FP32 (see WarpF16)
     float c[HD / 32][4];
-    const uint32_t kbase = slot + (lane >> 2) * kPitch + (lane & 3) * 4;
+    const float* kbase =
+        reinterpret_cast<const float*>(slot + (lane >> 2) * kPitch) + (lane & 3);
 #pragma unroll
     for (int j = 0; j < HD / 32; ++j) {
       c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
@@ -455,8 +453,8 @@ struct WarpF32 {
         const int ks = 4 * j + i;
         const uint4 a = s_q[ks * 32 + lane];
         uint32_t h0, l0, h1, l1;
-        split_tf32(lds_f32(kbase + ks * 32), h0, l0);
-        split_tf32(lds_f32(kbase + ks * 32 + 16), h1, l1);
+        split_tf32(kbase[ks * 8], h0, l0);
+        split_tf32(kbase[ks * 8 + 4], h1, l1);
         mma_tf32(c[j], a, h0, h1);
         mma_tf32(c[j], a, l0, l1);
       }
@@ -494,17 +492,17 @@ struct WarpF32 {
     uint4 pa;  // k index lane & 3: row 2 (lane & 3); + 4: the row after it
     split_tf32(p0, pa.x, pa.y);
     split_tf32(p1, pa.z, pa.w);
-    const uint32_t vbase = slot + kUnit * kPitch + 2 * (lane & 3) * kPitch + (lane >> 2) * 8;
+    const float2* vbase = reinterpret_cast<const float2*>(
+                              slot + kUnit * kPitch + 2 * (lane & 3) * kPitch) + (lane >> 2);
 #pragma unroll
     for (int j = 0; j < HD / 16; ++j) {
-      float v0[2], v1[2];  // this lane's two columns of its two rows
-      lds_f32x2(vbase + j * 64, v0);
-      lds_f32x2(vbase + kPitch + j * 64, v1);
+      // this lane's two columns of its two rows
+      const float2 v0 = vbase[j * 8], v1 = vbase[j * 8 + kPitch / 8];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint32_t h0, l0, h1, l1;
-        split_tf32(v0[i], h0, l0);
-        split_tf32(v1[i], h1, l1);
+        split_tf32(i ? v0.y : v0.x, h0, l0);
+        split_tf32(i ? v1.y : v1.x, h1, l1);
         mma_tf32(o[2 * j + i], pa, h0, h1);
         mma_tf32(o[2 * j + i], pa, l0, l1);
       }
@@ -659,7 +657,7 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
         cp_async_wait<kStages - 1>();
         __syncwarp();  // the unit is here for every lane
         if (row_of[s] >= 0)
-          w.template step<WEIGHTS>(ring + s * kSlot, n - row_of[s], scores + row_of[s],
+          w.template step<WEIGHTS>(s_ring + (warp * kStages + s) * kSlot, n - row_of[s], scores + row_of[s],
                                    p.score_pitch, G, s_q, lane);
         __syncwarp();  // and read out by every lane
         fetch(s, i0 + s + kStages, next_id);
