@@ -7,11 +7,16 @@
 // row), and their weights with them.  Rows carry their RoPE'd keys, so
 // attention over the kept rows needs no positions.
 //
-// Which rows: a cluster of CTAs a (sequence, kv head) selects over the weights
-// with the radix selection of cache_ops.cuh and writes the ascending list.
-// The rows then move in a second kernel (HBM-bound, each kept row read and
-// written once): to another cache, every (row, 16-byte chunk) by itself; in
-// place, in rounds (below).
+// Which rows: one CTA a (sequence, kv head), past 32,768 rows a cluster, selects over
+// the weights with the radix selection of cache_ops.cuh, its keys in shared memory,
+// and writes the ascending list.  The rows then move in a second kernel (HBM-bound,
+// each kept row read and written once): to another cache, every (row, 16-byte chunk)
+// by itself; in place, in rounds (below).
+//
+// Measured on one B200: 4096 rows of 8 kv heads to 1024, FP32, 10.3 us (two launches,
+// each a chain of loads); 16 sequences of up to 32,768 FP16 rows to 4096 110 us, 21
+// the selection (the longest sequence's walks) and 87 the copy (6.2 TB/s read and
+// written).
 #include "cache_ops.cuh"
 
 namespace gla {

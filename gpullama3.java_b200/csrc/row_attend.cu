@@ -5,19 +5,20 @@
 //   xb_h = sum_t p_ht v_t,  p_ht = exp(scale q_h.k_t - m_h) / l_h,
 //   w[g][t] += sum over the q heads h of kv head g of p_ht.
 //
-// HBM-bound: every listed row of K and V is read once for all G <= 8 q heads
-// of its kv head.  One cluster of S CTAs works on one (sequence, kv head); the
-// rows are dealt in units of 16 (FP16) or 8 (FP32) to the cluster's warps,
-// round robin.  A block is a multiple of 16 rows, so a unit lies in one block,
-// and a listed block costs one id lookup a unit.  Each warp streams its units
-// through a ring of its own in shared memory (cp.async, 16 bytes a lane, rows
-// past the last one zero-filled and never read) and keeps its own running
-// maximum, sum and output: no block barrier inside the stream.  The warps join
-// in shared memory and the CTAs through the cluster's shared memory, in a
-// fixed order, so results do not depend on timing, and there is no workspace,
-// counter or second launch (but see split_parts).  Rows in shared memory are padded by 16 bytes: a
-// row's pitch is an odd number of 16-byte chunks, which keeps ldmatrix and the
-// vector loads free of bank conflicts.
+// HBM-bound: every listed row of K and V is read once for all G <= 8 q heads of
+// its kv head.  One cluster of S CTAs works on one (sequence, kv head); the rows
+// are dealt in units of 16 (FP16) or 8 (FP32) to the cluster's warps, round robin.
+// A block is a multiple of 16 rows, so a unit lies in one block, and a listed block
+// costs one id lookup a unit.  Each warp streams its units through a ring of its own
+// in shared memory (cp.async, 16 bytes a lane, rows past the last one zero-filled
+// and never read) and keeps its own running maximum, sum and output: no block
+// barrier inside the stream.  The warps join in shared memory and the CTAs through
+// the cluster's shared memory, in a fixed order, so results do not depend on timing,
+// and listed blocks need no workspace, counter or second launch.  Rows in shared
+// memory are padded by 16 bytes: a row's pitch is an odd number of 16-byte chunks,
+// which keeps ldmatrix and the vector loads free of bank conflicts.  (One bulk copy
+// a row instead of 16 cp.async a lane: 320 us against 244 for 256 queries over
+// listed blocks; the copy engine takes short pieces more slowly.)
 //
 // FP16 cache: mma.sync.m16n8k16.  The 16 rows of A hold the high halves of the
 // (up to 8) q heads and their low halves, x - float(hi(x)): the two products
@@ -27,16 +28,23 @@
 // (p <= 1; a weight of 2^-17 still has all 22 bits).  tcgen05 has no place
 // here: 8 rows of a 128-row tile, and the stream is HBM-bound.
 // FP32 cache: the same with mma.sync.m16n8k8 on TF32 halves (split_tf32) of q and p
-// (the two row halves of A) and of K and V (two products).  On the CUDA cores a unit of 8 rows and 8 heads took about 600
-// instructions, this way about 330, whatever the group.
-// Rows are taken to be finite: an infinite key or value makes lo a NaN.
+// (the two row halves of A) and of K and V (two products).  On the CUDA cores a unit
+// of 8 rows and 8 heads took about 600 instructions, this way about 330, whatever the
+// group (16 sequences of 77 to 8191 rows, groups of 8: 47 us and 36).
+// Rows are taken to be finite: an infinite key or value makes a half a NaN.
 //
-// Weights: the normalisation is known only when all rows were seen, so the
-// scores (log2 units) go to a workspace, G floats a row against 2 head_dim
-// elements of K and V (read with an evict-first hint, so the scores stay in L2),
-// and are read again to add the weights.  Long sequences: the rows are cut into
-// parts of equal size, one CTA each, so that a ragged batch still fills the
-// device evenly, and a second kernel joins the parts and adds the weights.
+// Weights: the normalisation is known only when all rows were seen, so the scores
+// (log2 units) go to a workspace, G floats a row against 2 head_dim elements of K
+// and V (read with an evict-first hint, so the scores stay in L2), and are read again
+// to add the weights.  Long sequences: the rows are cut into parts of equal size, one
+// CTA each, so that a ragged batch still fills the device evenly, and a second kernel
+// joins the parts and adds the weights (part_rows_for).
+//
+// Measured on one B200: listed blocks, 64 of 64 FP16 rows for 4 kv heads of 128
+// 8.6 us (latency: 131 KB an SM through 64 bytes a clock, then the joins); 256
+// queries over one cache of 32,768 rows, 32 blocks each, 212 us (2.1 GB through L2,
+// 10 TB/s); 64 separate FP16 caches 107 us, 5.0 TB/s.  Weights, 131,072 FP16 rows of
+// 4 kv heads 60 us (4.6 TB/s with scores and weights).
 #include <cmath>
 
 #include "cache_ops.cuh"
@@ -301,14 +309,17 @@ struct WarpF16 {
       // (1.5e-6 of the output over 131,072 rows; 0.7e-6 this way), and waited longer
       float c[HD / 32][4];
       const uint32_t base = slot + (nt * 8 + in) * kPitch + sub * 16;
+      // (products of one accumulator apart: a product waits 21 clocks for the last)
+      uint32_t bk[HD / 32][4];
 #pragma unroll
       for (int j = 0; j < HD / 32; ++j) {
         c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
-        uint32_t b[4];
-        ldmatrix_x4(b, base + j * 64);
-        mma_f16(c[j], qa[2 * j], b[0], b[1]);
-        mma_f16(c[j], qa[2 * j + 1], b[2], b[3]);
+        ldmatrix_x4(bk[j], base + j * 64);
       }
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) mma_f16(c[j], qa[2 * j], bk[j][0], bk[j][1]);
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) mma_f16(c[j], qa[2 * j + 1], bk[j][2], bk[j][3]);
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int r = nt * 8 + 2 * (lane & 3) + j;
@@ -446,18 +457,22 @@ struct WarpF32 {
     const float* kbase =
         reinterpret_cast<const float*>(slot + (lane >> 2) * kPitch) + (lane & 3);
 #pragma unroll
-    for (int j = 0; j < HD / 32; ++j) {
-      c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
+    for (int j = 0; j < HD / 32; ++j) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) {
+      uint4 a[HD / 32];
+      uint32_t l0[HD / 32], l1[HD / 32];
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) {
         const int ks = 4 * j + i;
-        const uint4 a = s_q[ks * 32 + lane];
-        uint32_t h0, l0, h1, l1;
-        split_tf32(kbase[ks * 8], h0, l0);
-        split_tf32(kbase[ks * 8 + 4], h1, l1);
-        mma_tf32(c[j], a, h0, h1);
-        mma_tf32(c[j], a, l0, l1);
+        uint32_t h0, h1;
+        a[j] = s_q[ks * 32 + lane];
+        split_tf32(kbase[ks * 8], h0, l0[j]);
+        split_tf32(kbase[ks * 8 + 4], h1, l1[j]);
+        mma_tf32(c[j], a[j], h0, h1);
       }
+#pragma unroll
+      for (int j = 0; j < HD / 32; ++j) mma_tf32(c[j], a[j], l0[j], l1[j]);
     }
     float s[2];
 #pragma unroll
@@ -495,17 +510,22 @@ struct WarpF32 {
     const float2* vbase = reinterpret_cast<const float2*>(
                               slot + kUnit * kPitch + 2 * (lane & 3) * kPitch) + (lane >> 2);
 #pragma unroll
-    for (int j = 0; j < HD / 16; ++j) {
-      // this lane's two columns of its two rows
-      const float2 v0 = vbase[j * 8], v1 = vbase[j * 8 + kPitch / 8];
+    for (int j = 0; j < HD / 16; j += 2) {
+      uint32_t lo[4][2];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t h0, l0, h1, l1;
-        split_tf32(i ? v0.y : v0.x, h0, l0);
-        split_tf32(i ? v1.y : v1.x, h1, l1);
-        mma_tf32(o[2 * j + i], pa, h0, h1);
-        mma_tf32(o[2 * j + i], pa, l0, l1);
+      for (int e = 0; e < 2; ++e) {
+        // this lane's two columns of its two rows
+        const float2 v0 = vbase[(j + e) * 8], v1 = vbase[(j + e) * 8 + kPitch / 8];
+        uint32_t h0, h1;
+        split_tf32(v0.x, h0, lo[2 * e][0]);
+        split_tf32(v1.x, h1, lo[2 * e][1]);
+        mma_tf32(o[2 * (j + e)], pa, h0, h1);
+        split_tf32(v0.y, h0, lo[2 * e + 1][0]);
+        split_tf32(v1.y, h1, lo[2 * e + 1][1]);
+        mma_tf32(o[2 * (j + e) + 1], pa, h0, h1);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) mma_tf32(o[2 * j + e], pa, lo[e][0], lo[e][1]);
     }
   }
 

@@ -151,6 +151,12 @@ def _ptr(x) -> int | None:
     raise TypeError(f"expected a device tensor or an address, got {type(x)!r}")
 
 
+def _ptrs(*xs):
+    """_ptr of every argument: one call for a whole argument list."""
+    return [x if x is None or x.__class__ is int else
+            (x.data_ptr() if hasattr(x, "data_ptr") else _ptr(x)) for x in xs]
+
+
 def device_view(address: int, shape, dtype):
     """A torch CUDA tensor viewing `address` (device memory the library
     allocated, e.g. a KV cache from gla_kv_cache_alloc) without copying; it
@@ -452,9 +458,9 @@ class Context:
         if kv_stride is None:
             kv_stride = n_kv_heads * head_dim
         fn = self._L.gla_block_bounds_f16kv if f16_cache else self._L.gla_block_bounds_f32kv
-        self._check(fn(self._h, _ptr(k_ptrs), _ptr(start_pos), _ptr(n_pos), max_n_pos,
-                       _ptr(bounds_ptrs), batch, n_kv_heads, head_dim, kv_stride, block_rows),
-                    "gla_block_bounds")
+        k, s, n, b = _ptrs(k_ptrs, start_pos, n_pos, bounds_ptrs)
+        self._check(fn(self._h, k, s, n, max_n_pos, b, batch, n_kv_heads, head_dim, kv_stride,
+                       block_rows), "gla_block_bounds")
 
     def rope_append_batched(self, q, k, v, q_out, k_ptrs, v_ptrs, positions, batch, n_heads,
                             n_kv_heads, head_dim, context_length, theta, style=ROPE_INTERLEAVED,
@@ -465,18 +471,18 @@ class Context:
             kv_stride = n_kv_heads * head_dim
         fn = (self._L.gla_rope_append_batched_f16kv if f16_cache
               else self._L.gla_rope_append_batched_f32kv)
-        self._check(fn(self._h, _ptr(q), _ptr(k), _ptr(v), _ptr(q_out), _ptr(k_ptrs),
-                       _ptr(v_ptrs), _ptr(positions), _ptr(rows), _ptr(bounds_ptrs), block_rows,
-                       batch, n_heads, n_kv_heads, head_dim, kv_stride, context_length, theta,
-                       style), "gla_rope_append_batched")
+        self._check(fn(self._h, *_ptrs(q, k, v, q_out, k_ptrs, v_ptrs, positions, rows,
+                                       bounds_ptrs), block_rows, batch, n_heads, n_kv_heads,
+                       head_dim, kv_stride, context_length, theta, style),
+                    "gla_rope_append_batched")
 
     def block_select(self, q, bounds_ptrs, n_pos, max_n_pos, block_ids, batch, n_heads,
                      n_kv_heads, head_dim, block_rows, n_sel, n_first=0, n_last=1,
                      f16_cache=False):
         """gla_block_select_*: ids of the blocks each query's kv heads read."""
         fn = self._L.gla_block_select_f16kv if f16_cache else self._L.gla_block_select_f32kv
-        self._check(fn(self._h, _ptr(q), _ptr(bounds_ptrs), _ptr(n_pos), max_n_pos,
-                       _ptr(block_ids), batch, n_heads, n_kv_heads, head_dim, block_rows, n_sel,
+        q, bounds, n, ids = _ptrs(q, bounds_ptrs, n_pos, block_ids)
+        self._check(fn(self._h, q, bounds, n, max_n_pos, ids, batch, n_heads, n_kv_heads, head_dim, block_rows, n_sel,
                        n_first, n_last), "gla_block_select")
 
     def decode_blocks(self, q, k_ptrs, v_ptrs, n_pos, block_ids, n_sel, xb, batch, n_heads,
@@ -488,8 +494,8 @@ class Context:
         if kv_stride is None:
             kv_stride = n_kv_heads * head_dim
         fn = self._L.gla_decode_blocks_f16kv if f16_cache else self._L.gla_decode_blocks_f32kv
-        self._check(fn(self._h, _ptr(q), _ptr(k_ptrs), _ptr(v_ptrs), _ptr(n_pos),
-                       _ptr(block_ids), n_sel, _ptr(xb), batch, n_heads, n_kv_heads, head_dim,
+        q, k, v, n, ids, xb = _ptrs(q, k_ptrs, v_ptrs, n_pos, block_ids, xb)
+        self._check(fn(self._h, q, k, v, n, ids, n_sel, xb, batch, n_heads, n_kv_heads, head_dim,
                        kv_stride, block_rows, scale), "gla_decode_blocks")
 
     def decode_weights(self, q, k_ptrs, v_ptrs, n_pos, max_n_pos, xb, weight_ptrs, weight_stride,
@@ -501,8 +507,8 @@ class Context:
         if kv_stride is None:
             kv_stride = n_kv_heads * head_dim
         fn = self._L.gla_decode_weights_f16kv if f16_cache else self._L.gla_decode_weights_f32kv
-        self._check(fn(self._h, _ptr(q), _ptr(k_ptrs), _ptr(v_ptrs), _ptr(n_pos), max_n_pos,
-                       _ptr(xb), _ptr(weight_ptrs), weight_stride, batch, n_heads, n_kv_heads,
+        q, k, v, n, xb, w = _ptrs(q, k_ptrs, v_ptrs, n_pos, xb, weight_ptrs)
+        self._check(fn(self._h, q, k, v, n, max_n_pos, xb, w, weight_stride, batch, n_heads, n_kv_heads,
                        head_dim, kv_stride, scale), "gla_decode_weights")
 
     def kv_evict(self, k_ptrs, v_ptrs, weight_ptrs, weight_stride, n_pos, max_n_pos, n_keep,
@@ -513,7 +519,8 @@ class Context:
         if kv_stride is None:
             kv_stride = n_kv_heads * head_dim
         fn = self._L.gla_kv_evict_f16kv if f16_cache else self._L.gla_kv_evict_f32kv
-        self._check(fn(self._h, _ptr(k_ptrs), _ptr(v_ptrs), _ptr(weight_ptrs), weight_stride,
-                       _ptr(n_pos), max_n_pos, n_keep, n_recent, _ptr(kept), _ptr(k_out_ptrs),
-                       _ptr(v_out_ptrs), _ptr(weight_out_ptrs), weight_out_stride, batch,
-                       n_kv_heads, head_dim, kv_stride), "gla_kv_evict")
+        k, v, w, n, kept, ko, vo, wo = _ptrs(k_ptrs, v_ptrs, weight_ptrs, n_pos, kept, k_out_ptrs,
+                                             v_out_ptrs, weight_out_ptrs)
+        self._check(fn(self._h, k, v, w, weight_stride, n, max_n_pos, n_keep, n_recent, kept, ko,
+                       vo, wo, weight_out_stride, batch, n_kv_heads, head_dim, kv_stride),
+                    "gla_kv_evict")

@@ -500,7 +500,7 @@ int32_t gla_rope_append_f32(gla_ctx* ctx, float* q, float* k, const float* v, fl
  *  - n_pos: DEVICE int32 [batch], the rows a sequence has, 0 to max_n_pos (host).
  *    A value outside is clamped and latches GLA_ERR_INVALID_ARG in the device
  *    status.  Rows at and past n_pos are never read nor written, so what they
- *    hold (an infinity, a NaN) does not matter.
+ *    hold (an infinity, a NaN) does not matter.  Attended rows must be finite.
  *  - block_rows (16, 32, 64 or 128): block j is rows [j*block_rows, (j+1)*block_rows).
  *  - Results do not depend on timing: two calls on the same input give the
  *    same bits.
@@ -556,9 +556,9 @@ int32_t gla_rope_append_batched_f16kv(gla_ctx* ctx, const float* q, const float*
  *     score(j, g) = max over the q heads h of g of sum_d max(q_hd lo_jgd, q_hd hi_jgd),
  * an upper bound of q_h . k_t over block j's rows (for a positive scale; lo <= hi, as
  * gla_block_bounds_* gives them).  The order is that of the sums in FP64: the highest
- * are chosen, ties to the lowest block, a head whose sum is NaN counts as the lowest.  With n_blocks <= n_sel all are
- * chosen.  max_n_pos / block_rows, rounded up, at most 24576 (else
- * GLA_ERR_NOT_SUPPORTED).  Batch entries may share bounds: the queries of
+ * are chosen, ties to the lowest block, a head whose sum is NaN counts as the lowest.
+ * With n_blocks <= n_sel all are chosen.  max_n_pos / block_rows, rounded up, at most
+ * 24576 (else GLA_ERR_NOT_SUPPORTED).  Batch entries may share bounds: the queries of
  * a prompt chunk over one cache, each with its own n_pos and blocks. */
 int32_t gla_block_select_f32kv(gla_ctx* ctx, const float* q, const float* const* bounds_ptrs,
                                const int32_t* n_pos, int32_t max_n_pos, int32_t* block_ids,
@@ -593,8 +593,8 @@ int32_t gla_decode_blocks_f16kv(gla_ctx* ctx, const float* q, const uint16_t* co
  * w = weight_ptrs[b], FP32 [n_kv_heads][weight_stride], weight_stride >= max_n_pos.
  * Entries at and past n_pos are left as they were; set a row's entry to 0 when the
  * row is appended.  Batch entries must not share weights.  Uses a context workspace
- * of batch * n_heads * max_n_pos floats, grown on first use (not during stream
- * capture). */
+ * of batch * n_heads * max_n_pos floats, and about as much again for short sequences
+ * of a few heads, grown on first use (not during stream capture). */
 int32_t gla_decode_weights_f32kv(gla_ctx* ctx, const float* q, const float* const* k_ptrs,
                                  const float* const* v_ptrs, const int32_t* n_pos,
                                  int32_t max_n_pos, float* xb, float* const* weight_ptrs,
