@@ -86,8 +86,9 @@ __device__ __forceinline__ float coefficient(float q, bool is_lo) {
 // kChunks 16-byte chunks, lo then hi, over kLanes lanes; a lane holds the
 // coefficients of its chunks in registers (at most 8 elements of GP heads) and
 // a lane group scores kBlk blocks at once, so that one reduce_scatter joins
-// them.  The blocks come through a ring of each warp's own in shared memory
-// (cp.async), kStages steps deep: a step's latency is most of its time.
+// them.  The blocks come through a ring of each warp's own in shared memory, kStages
+// steps deep, by one bulk copy a block: its 256 to 1024 bytes lie together, and
+// copies by 16 bytes a lane compete with the lanes' own shared memory traffic.
 template <class T, int HD, int GP>
 struct Shape {
   static constexpr int kPer = 16 / sizeof(T);
@@ -99,7 +100,7 @@ struct Shape {
   static constexpr int kBlk = kWant * GP > kLanes ? kLanes / GP : kWant;  // a value a lane
   static constexpr int kVals = kBlk * GP;
   static constexpr int kSlot = kSub * kBlk * kChunks * 16;  // bytes of a step
-  static constexpr int kStages = 72 * 1024 / (kWarps * kSlot) > 4 ? 4 : 72 * 1024 / (kWarps * kSlot);
+  static constexpr int kStages = std::min(6, 96 * 1024 / (kWarps * kSlot));
   static constexpr int kRing = kWarps * kStages * kSlot;
   static_assert(kCpl * kPer <= 8, "the error bound counts 8 terms a lane");
   static_assert(kStages >= 2, "a step in flight beside the one at work");
@@ -110,10 +111,6 @@ template <class T, int HD, int GP>
 size_t select_smem(int64_t max_nb) {  // max_nb: a multiple of 4
   using Sh = Shape<T, HD, GP>;
   return (size_t)std::max<int64_t>(Sh::kRing, max_nb * 4) + (size_t)max_nb * 4;
-}
-
-__device__ __forceinline__ void cp_async_chunk(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // The FP64 score of one (block, kv head), by one warp: the larger product of
@@ -164,11 +161,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   __shared__ int32_t s_near[kNear];
   __shared__ uint64_t s_near_key[kNear];
   __shared__ int32_t s_near_n, s_sure_n;
+  __shared__ uint64_t s_bar[kWarps * Sh::kStages];
+  __shared__ int s_abort;  // a bounded wait gave up
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = S > 1 ? (int)(blockIdx.x % (unsigned)S) : 0;
   const int item = (int)(blockIdx.x / (unsigned)S);
   const int b = item / n_kv, g = item - b * n_kv;
   const int G = n_heads / n_kv;
+  if (tid == 0) s_abort = 0;
   pdl_wait();
   pdl_launch_dependents();
   // q, the length and the pointer are loaded side by side
@@ -199,22 +199,22 @@ __global__ void __launch_bounds__(kThreads, 2)
   const T* base = bounds + (int64_t)n_first * row + (int64_t)g * 2 * HD;
   uint32_t* s_upper = reinterpret_cast<uint32_t*>(s_dyn);
   uint32_t* s_lower = reinterpret_cast<uint32_t*>(s_dyn + max(Sh::kRing, max_nb * 4));
-  const uint32_t ring = smem_u32(s_dyn) + warp * (kStages * Sh::kSlot) + sub * (Sh::kSlot / Sh::kSub);
-  auto fetch = [&](int s, int32_t jw) {  // blocks jw + sub * kBlk + 0 .. kBlk - 1
-    if (jw < hi) {
+  char* ring = s_dyn + warp * (kStages * Sh::kSlot);
+  uint64_t* bars = s_bar + warp * kStages;  // a slot's copies have landed
+  if (lane == 0) {
 #pragma unroll
-      for (int i = 0; i < kBlk; ++i) {
-        const T* src = base + (int64_t)min(jw + sub * kBlk + i, hi - 1) * row;
-#pragma unroll
-        for (int c = 0; c < kCpl; ++c) {
-          const int chunk = sl + c * kLanes;
-          if (chunk < Sh::kChunks)
-            cp_async_chunk(ring + s * Sh::kSlot + (i * Sh::kChunks + chunk) * 16,
-                           reinterpret_cast<const float4*>(src) + chunk);
-        }
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int s = 0; s < kStages; ++s) mbar_init(bars + s, 1);
+    fence_mbarrier_init();
+  }
+  __syncwarp();
+  constexpr int kBytes = Sh::kChunks * 16;  // of a block
+  auto fetch = [&](int s, int32_t jw) {  // blocks jw + 0 .. kSub * kBlk - 1, a lane each
+    if (jw >= hi) return;
+    if (lane == 0) mbar_arrive_expect_tx(bars + s, Sh::kSlot);
+    __syncwarp();
+    if (lane < Sh::kSub * kBlk)  // (the last block again past the end)
+      bulk_g2s_keep(ring + s * Sh::kSlot + lane * kBytes,
+                    base + (int64_t)min(jw + lane, hi - 1) * row, kBytes, bars + s);
   };
   const int32_t w0 = lo + warp * Sh::kSub * kBlk;  // the warp's first block
   // in flight while the coefficients are set up
@@ -249,13 +249,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   float big = 0.f;
   bool strange = false;  // a NaN bound (its scores are NaN; a maximum would drop it)
   uint32_t kmin = ~0u, kmax = 0;
-  for (int32_t jw0 = w0; jw0 < hi; jw0 += kStages * kStep) {
+  uint32_t phase = 0;  // parity of the ring's round
+  for (int32_t jw0 = w0; jw0 < hi; jw0 += kStages * kStep, phase ^= 1) {
 #pragma unroll
     for (int st = 0; st < kStages; ++st) {
       const int32_t jw = jw0 + st * kStep, j0 = jw + sub * kBlk;
       if (jw >= hi) break;
-      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-      __syncwarp();
+      mbar_wait(bars + st, phase, &s_abort, status);
       float acc[kVals];
 #pragma unroll
       for (int i = 0; i < kBlk; ++i) {
@@ -267,9 +267,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           const int chunk = sl + c * kLanes;
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
           if (chunk < Sh::kChunks)
-            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                         : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                         : "r"(ring + st * Sh::kSlot + (i * Sh::kChunks + chunk) * 16));
+            x = reinterpret_cast<const float4*>(ring + st * Sh::kSlot +
+                                                (sub * kBlk + i) * kBytes)[chunk];
 #pragma unroll
           for (int p = 0; p < kPer; ++p) {
             const float y = (float)reinterpret_cast<const T*>(&x)[p];

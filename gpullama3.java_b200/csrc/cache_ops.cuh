@@ -168,6 +168,17 @@ int launch_clusters(void (*kern)(Params...), unsigned grid, int threads, size_t 
   return GLA_OK;
 }
 
+// Bulk copy global -> shared (bulk_g2s without its evict-first hint: data that is
+// read again, by the other queries of a chunk or at the next token).
+__device__ __forceinline__ void bulk_g2s_keep(void* dst, const void* src, uint32_t bytes,
+                                              uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // Order-preserving maps of a score to an unsigned key: a larger score has the
 // larger key, -0 equals +0, and a NaN has the lowest key, 0.
 __device__ __forceinline__ uint64_t order_key(double x) {

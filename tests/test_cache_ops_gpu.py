@@ -869,3 +869,137 @@ def test_select_over_the_most_blocks(gla_ctx, t):
     want, gap = select64(q[0], bs, nb * br - 3, br, n_sel, 2, 3)
     assert gap > 1e-11
     np.testing.assert_array_equal(ids[0].cpu().numpy(), want)
+
+
+# ------------------------------------------------------------------------- calls side by side
+def test_two_contexts_at_once(gla_ctx):
+    """Two contexts on two streams, their calls in flight together, give what each gives alone."""
+    g, nh, n_kv, hd, n = rng(23), 8, 2, 64, 6000
+    got, alone = [], []
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    data = []
+    for _ in range(2):
+        k, v = caches(g, [n], n_kv, hd, "f16"), caches(g, [n], n_kv, hd, "f16")
+        data.append((normal(g, 1, nh, hd), k, v, ptrs(k), ptrs(v), i32([n])))
+    torch.cuda.synchronize()
+    for together in (False, True):
+        out = []
+        ctxs = [gla.Context(0, s.cuda_stream) for s in streams]
+        for rep in range(3):
+            for ctx, s, (q, k, v, kp, vp, np_) in zip(ctxs, streams, data):
+                with torch.cuda.stream(s):
+                    if rep == 0:
+                        out.append((torch.empty(1, nh, hd, device="cuda"), torch.zeros(n_kv, n, device="cuda")))
+                    xb, w = out[ctxs.index(ctx)]
+                    ctx.decode_weights(q, kp, vp, np_, n, xb, ptrs([w]), n, 1, nh, n_kv, hd, f16_cache=True)
+                if not together:
+                    torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        for ctx in ctxs:
+            assert ctx.device_status() == 0
+            ctx.close()
+        (got if together else alone).extend(out)
+    for a, b in zip(alone, got):
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_more_sequences_than_a_grid_row(gla_ctx):
+    """70,000 sequences of one and two rows."""
+    batch, nh, n_kv, hd, br, cap = 70000, 2, 1, 64, 16, 2
+    g = rng(24)
+    kv = normal(g, 2, batch, cap, hd)
+    at = torch.arange(batch, device="cuda", dtype=torch.int64) * (cap * hd * 4)
+    kp, vp = kv[0].data_ptr() + at, kv[1].data_ptr() + at
+    q, k, v = normal(g, batch, nh, hd), normal(g, batch, n_kv, hd), normal(g, batch, n_kv, hd)
+    rows = (torch.arange(batch, device="cuda") % 2).int()
+    q_out = torch.empty_like(q)
+    zero = torch.zeros_like(rows)
+    gla_ctx.rope_append_batched(q, k, v, q_out, kp, vp, zero, batch, nh, n_kv, hd, cap, 1e4, rows=rows)
+    pick = torch.arange(batch, device="cuda")
+    # position 0 turns nothing
+    assert torch.equal(q_out, q) and torch.equal(kv[0][pick, rows.long()], k[:, 0])
+    bounds = torch.zeros(batch, 2, hd, device="cuda")
+    bp = bounds.data_ptr() + torch.arange(batch, device="cuda", dtype=torch.int64) * (2 * hd * 4)
+    n = rows + 1
+    gla_ctx.block_bounds(kp, n, cap, bp, batch, n_kv, hd, br)
+    two = (rows == 1)[:, None]
+    assert torch.equal(bounds[:, 0], torch.where(two, kv[0].amin(1), kv[0][:, 0]))
+    ids = torch.full((batch, n_kv, 1), 9, dtype=torch.int32, device="cuda")
+    gla_ctx.block_select(q, bp, n, cap, ids, batch, nh, n_kv, hd, br, 1)
+    assert (ids == 0).all()
+    xb = torch.empty(batch, nh, hd, device="cuda")
+    gla_ctx.decode_blocks(q, kp, vp, n, ids, 1, xb, batch, nh, n_kv, hd, br)
+    ok(gla_ctx)
+    s = torch.einsum("bhd,btd->bht", q.double(), kv[0].double()) / 8
+    s[~two[:, 0], :, 1] = -math.inf
+    want = torch.einsum("bht,btd->bhd", torch.softmax(s, -1), kv[1].double())
+    # two rows of |q| and |k| below 6: attention_bound's terms at its largest
+    tol = attention_bound(torch.full((1, hd), 6.0, device="cuda"), torch.full((2, hd), 6.0, device="cuda"),
+                          torch.full((2, hd), 6.0, device="cuda"), 1 / 8)[0]
+    assert float(kv.abs().max()) < 6 and float(q.abs().max()) < 6
+    assert float((xb.double() - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("t", TYPES)
+def test_eviction_captured_and_replayed(gla_ctx, t):
+    """Weights, eviction in place and bounds in one captured graph, replayed while the caches
+    grow again: every replay keeps what the 64-bit order keeps of its own weights."""
+    f16, g = t == "f16", rng(25)
+    nh, n_kv, hd, br, cap, keep, recent, theta = 4, 2, 96, 32, 300, 100, 11, 1e4
+    k = [normal(g, cap, n_kv * hd).to(DT[t]) for _ in range(2)]
+    v = [normal(g, cap, n_kv * hd).to(DT[t]) for _ in range(2)]
+    w = [torch.zeros(n_kv, cap, device="cuda") for _ in range(2)]
+    bs = [torch.zeros(-(-cap // br), n_kv, 2, hd, dtype=DT[t], device="cuda") for _ in range(2)]
+    kp, vp, wp, bp = ptrs(k), ptrs(v), ptrs(w), ptrs(bs)
+    q, xb = normal(g, 2, nh, hd), torch.empty(2, nh, hd, device="cuda")
+    n = i32([280, 90])
+    left = torch.clamp(n, max=keep)
+    kept = torch.empty(2, n_kv, keep, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    ctx = gla.Context(0, stream.cuda_stream)
+
+    def step():
+        ctx.decode_weights(q, kp, vp, n, cap, xb, wp, cap, 2, nh, n_kv, hd, f16_cache=f16)
+        ctx.kv_evict(kp, vp, wp, cap, n, cap, keep, recent, kept, 2, n_kv, hd, f16_cache=f16)
+        torch.clamp(n, max=keep, out=left)
+        ctx.block_bounds(kp, left, cap, bp, 2, n_kv, hd, br, f16_cache=f16)
+
+    with torch.cuda.stream(stream):
+        ctx.decode_weights(q, kp, vp, i32([0, 0]), cap, xb, wp, cap, 2, nh, n_kv, hd, f16_cache=f16)
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+        for lens in ([280, 90], [131, 90], [300, 101], [100, 100]):
+            n.copy_(i32(lens))
+            q.normal_(generator=g)
+            k0, w0 = [x.clone() for x in k], [x.clone() for x in w]
+            graph.replay()
+            for b, m in enumerate(lens):
+                kk, vv = rows_of(k0[b], m, n_kv, hd), None
+                for h in range(n_kv):
+                    grp = nh // n_kv
+                    qh = q[b, h * grp:(h + 1) * grp]
+                    _, p = attend64(qh, kk[:, h], kk[:, h], hd ** -0.5)
+                    rows = kept[b, h].tolist()
+                    rows = rows[: min(m, keep)]
+                    assert rows == sorted(set(rows)) and rows[-1] == m - 1
+                    total = w0[b][h, :m].double() + p
+                    # the kept weights are the sums' (see test_decode_weights_adds_the_softmax), and no
+                    # dropped row had more than a kept older one by over both sums' errors
+                    _, rel = attention_bound(qh, kk[:, h], kk[:, h], hd ** -0.5)
+                    off = 2 * float((rel * p + 2.0 ** -24 * total).max())
+                    assert float((w[b][h, : len(rows)].double() - total[rows]).abs().max()) <= off
+                    if m > keep:
+                        old = [r for r in rows if r < m - recent]
+                        gone = sorted(set(range(m - recent)) - set(old))
+                        assert float(total[old].min()) >= float(total[gone].max()) - off
+                        assert (w[b][h, keep:m] == 0).all()
+                    assert torch.equal(k[b][: len(rows), h * hd:(h + 1) * hd], k0[b][rows, h * hd:(h + 1) * hd])
+                x = rows_of(k[b], min(m, keep), n_kv, hd)
+                assert torch.equal(bs[b][0, :, 0], x[:br].amin(0)) and torch.equal(bs[b][-(-len(rows) // br) - 1, :, 1], x[(-(-len(rows) // br) - 1) * br:].amax(0))
+        assert ctx.device_status() == 0
+        del graph
+    stream.synchronize()
+    ctx.close()
