@@ -593,8 +593,8 @@ int32_t gla_decode_blocks_f16kv(gla_ctx* ctx, const float* q, const uint16_t* co
  * w = weight_ptrs[b], FP32 [n_kv_heads][weight_stride], weight_stride >= max_n_pos.
  * Entries at and past n_pos are left as they were; set a row's entry to 0 when the
  * row is appended.  Batch entries must not share weights.  Uses a context workspace
- * of batch * n_heads * max_n_pos floats, and about as much again for short sequences
- * of a few heads, grown on first use (not during stream capture). */
+ * of batch * n_heads * max_n_pos floats, and up to half as much again for the parts
+ * of long sequences, grown on first use (not during stream capture). */
 int32_t gla_decode_weights_f32kv(gla_ctx* ctx, const float* q, const float* const* k_ptrs,
                                  const float* const* v_ptrs, const int32_t* n_pos,
                                  int32_t max_n_pos, float* xb, float* const* weight_ptrs,
@@ -613,7 +613,8 @@ int32_t gla_decode_weights_f16kv(gla_ctx* ctx, const float* q, const uint16_t* c
  * for gla_decode_weights_*), ties to the lower row, a NaN lowest.  Kept rows keep their
  * order and become rows 0..n_keep-1 of that kv head; their weights move with them.
  * kept (DEVICE int32 [batch][n_kv_heads][n_keep]) receives the rows they were, -1 behind
- * the last.  A sequence with n_pos <= n_keep keeps all.  The caller goes on with
+ * the last.  A sequence with n_pos <= n_keep keeps all.  Batch entries must not share
+ * caches or weights that are written.  The caller goes on with
  * min(n_pos, n_keep) rows (and rebuilds the block bounds, if it uses them).
  *  - k_out_ptrs, v_out_ptrs and weight_out_ptrs all NULL: in place; weights of the
  *    rows [n_keep, n_pos) become 0, cache rows there are left as they were.

@@ -361,7 +361,7 @@ def test_decode_blocks_listed_twice_and_shared_caches(gla_ctx, t):
 
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("nh,n_kv,hd", HEADS)
-@pytest.mark.parametrize("lens", [[1, 0, 15, 16, 17, 300], [4000, 129], [30000]])
+@pytest.mark.parametrize("lens", [[1, 0, 15, 16, 17, 300], [4000, 129], [30000], [9001, 0, 1, 513]])
 def test_decode_weights_adds_the_softmax(gla_ctx, t, nh, n_kv, hd, lens):
     g, pad, top = rng(10, nh, hd, len(lens)), 8, max(lens)
     k, v = caches(g, lens, n_kv, hd, t, pad_cols=pad), caches(g, lens, n_kv, hd, t, pad_cols=pad)
