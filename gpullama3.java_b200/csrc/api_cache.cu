@@ -205,6 +205,27 @@ AttendRequest attend_request(gla_ctx* ctx, int dtype, const float* q, const void
   return r;
 }
 
+// Grows the attention workspace (scores, parts).  An outgrown buffer lives until gla_destroy:
+// kernels in flight and captured graphs may still use it.
+int ensure_scores(gla_ctx* ctx, size_t floats) {
+  if (floats <= ctx->scores_cap) return GLA_OK;
+  if (stream_capturing(ctx->stream))
+    return fail(ctx, GLA_ERR_INVALID_ARG,
+                "attention workspace must grow; run the largest call once before capture");
+  ctx->retired.reserve(ctx->retired.size() + 1);
+  // doubling bounds what outgrown buffers hold to the size of the current one
+  const size_t cap = std::max(floats, 2 * ctx->scores_cap);
+  void* p = nullptr;
+  if (cudaMalloc(&p, cap * sizeof(float)) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(ctx, GLA_ERR_OUT_OF_MEMORY, "attention workspace allocation failed");
+  }
+  if (ctx->scores) ctx->retired.push_back(ctx->scores);
+  ctx->scores = static_cast<float*>(p);
+  ctx->scores_cap = cap;
+  return GLA_OK;
+}
+
 int32_t decode_blocks(gla_ctx* ctx, int dtype, const float* q, const void* const* k_ptrs,
                       const void* const* v_ptrs, const int32_t* n_pos, const int32_t* block_ids,
                       int32_t n_sel, float* xb, int32_t batch,
@@ -226,30 +247,12 @@ int32_t decode_blocks(gla_ctx* ctx, int dtype, const float* q, const void* const
     r.block_ids = block_ids;
     r.n_sel = n_sel;
     r.block_rows = block_rows;
+    rc = ensure_scores(ctx, attend_workspace_floats(r, ctx->dev));
+    if (rc != GLA_OK) return rc;
+    r.scores = ctx->scores;
     std::string err;
     return finish(ctx, launch_attend(r, ctx->dev, ctx->stream, &err), err);
   });
-}
-
-// Grows the score workspace.  An outgrown buffer lives until gla_destroy:
-// kernels in flight and captured graphs may still use it.
-int ensure_scores(gla_ctx* ctx, size_t floats) {
-  if (floats <= ctx->scores_cap) return GLA_OK;
-  if (stream_capturing(ctx->stream))
-    return fail(ctx, GLA_ERR_INVALID_ARG,
-                "score workspace must grow; run the largest call once before capture");
-  ctx->retired.reserve(ctx->retired.size() + 1);
-  // doubling bounds what outgrown buffers hold to the size of the current one
-  const size_t cap = std::max(floats, 2 * ctx->scores_cap);
-  void* p = nullptr;
-  if (cudaMalloc(&p, cap * sizeof(float)) != cudaSuccess) {
-    cudaGetLastError();
-    return fail(ctx, GLA_ERR_OUT_OF_MEMORY, "score workspace allocation failed");
-  }
-  if (ctx->scores) ctx->retired.push_back(ctx->scores);
-  ctx->scores = static_cast<float*>(p);
-  ctx->scores_cap = cap;
-  return GLA_OK;
 }
 
 int32_t decode_weights(gla_ctx* ctx, int dtype, const float* q, const void* const* k_ptrs,
@@ -268,7 +271,7 @@ int32_t decode_weights(gla_ctx* ctx, int dtype, const float* q, const void* cons
                                      n_heads, n_kv_heads, head_dim, kv_stride, scale);
     r.weight_ptrs = weight_ptrs;
     r.weight_stride = weight_stride;
-    rc = ensure_scores(ctx, attend_score_floats(r, ctx->dev));
+    rc = ensure_scores(ctx, attend_workspace_floats(r, ctx->dev));
     if (rc != GLA_OK) return rc;
     r.scores = ctx->scores;
     std::string err;

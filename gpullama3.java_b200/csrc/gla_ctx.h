@@ -32,9 +32,9 @@ struct gla_ctx {
   gla::PeerExchange xch;            // sharded decode: peer exchange buffers
   int32_t opt_early_kv = 2;         // GLA_OPT_EARLY_KV_PREFETCH
   int32_t opt_shard_exchange = 1;   // GLA_OPT_SHARD_EXCHANGE
-  float* scores = nullptr;          // attention scores of gla_decode_weights_*
+  float* scores = nullptr;          // scores and parts (gla_decode_weights_*, _blocks_*)
   size_t scores_cap = 0;            // floats
-  std::vector<void*> retired;       // outgrown score buffers: captured graphs may still name them
+  std::vector<void*> retired;       // outgrown scores: captured graphs may still name them
   std::string last_error;
 };
 

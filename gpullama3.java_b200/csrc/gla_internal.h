@@ -200,10 +200,10 @@ struct AttendRequest {  // row_attend.cu
   int32_t block_rows = 0;
   float* const* weight_ptrs = nullptr;  // all rows, weights added: [n_kv][weight_stride] each
   int64_t weight_stride = 0;
-  float* scores = nullptr;              // workspace of attend_score_floats(...) floats
+  float* scores = nullptr;              // workspace of attend_workspace_floats(...) floats
   int32_t* status;
 };
-size_t attend_score_floats(const AttendRequest& r, const DeviceInfo& dev);
+size_t attend_workspace_floats(const AttendRequest& r, const DeviceInfo& dev);
 int launch_attend(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,
                   std::string* err);
 

@@ -155,7 +155,7 @@ struct AttendParams {
   int64_t score_pitch;
   float* part;        // o of the parts: [item][S][G][HD]
   float2* part_ml;    // their (m, l): [item][G][S]
-  int32_t part_rows;  // of a part
+  int32_t part_units;  // of a part
   int32_t* status;
 };
 
@@ -624,11 +624,14 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   auto id_of = [&](int32_t u) {
     return BLOCKS && u < listed ? __ldg(ids + (u >> (p.br_shift - kShift))) : -1;
   };
+  // units of this CTA's warps: a cluster's deal, or this part's
+  const int32_t cta_first = rank * (p.part ? p.part_units : kWarps);
+  const int32_t stride = p.part ? kWarps : S * kWarps;
   int32_t id[kStages + 1];
 #pragma unroll
-  for (int s = 0; s <= kStages; ++s) id[s] = id_of((rank + s * S) * kWarps + warp);
+  for (int s = 0; s <= kStages; ++s) id[s] = id_of(cta_first + s * stride + warp);
   int32_t n = clamped_rows(p.n_pos, b, p.max_n_pos, p.status);
-  if (WEIGHTS && p.part && (int64_t)rank * p.part_rows >= n) return;
+  if (WEIGHTS && p.part && (int64_t)rank * p.part_units * U >= n) return;
   const T* k = static_cast<const T*>(p.k_ptrs[b]);
   const T* v = static_cast<const T*>(p.v_ptrs[b]);
   if (!usable_ptrs(k, v, p.status)) n = 0;
@@ -636,14 +639,8 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   if (WEIGHTS && !usable_weights(wts, p.status)) n = 0;
   k += (int64_t)g * HD;
   v += (int64_t)g * HD;
-  // units of this CTA's warps: a cluster's deal, or this part's
   int32_t units = BLOCKS ? (n > 0 ? listed : 0) : (int32_t)(((int64_t)n + U - 1) / U);
-  int32_t cta_first = rank * kWarps, stride = S * kWarps;
-  if (WEIGHTS && p.part) {
-    cta_first = rank * (p.part_rows / U);
-    units = min(units, cta_first + p.part_rows / U);
-    stride = kWarps;
-  }
+  if (p.part) units = min(units, cta_first + p.part_units);
   const int32_t first = cta_first + warp;
   float* scores = WEIGHTS ? p.scores + (int64_t)item * G * p.score_pitch : nullptr;
 
@@ -747,7 +744,7 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
     }
     __syncthreads();
   };
-  if (WEIGHTS && p.part) {  // joined by attend_join_kernel
+  if (p.part) {  // joined by attend_join_kernel
     float* part = p.part + ((int64_t)item * S + rank) * G * HD;
     for (int i = tid; i < G * HD; i += kThreads) part[i] = cta_o(i);
     if (tid < G)
@@ -800,13 +797,13 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
 
 // Joins the parts of every item.  Of an item's CTAs the first `out_shares` add up
 // 32 outputs each, the others normalise kJoinRows rows' scores and add the
-// weights.  Latency-bound: everything that does not need the joined (m, l) is
+// weights (listed blocks have none: outputs only).  Latency-bound: everything that does not need the joined (m, l) is
 // loaded before they are known.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinRows = 512;
 
 __global__ void __launch_bounds__(kJoinThreads)
-    attend_join_kernel(const __grid_constant__ AttendParams p, int32_t head_dim,
+    attend_join_kernel(const __grid_constant__ AttendParams p, int32_t head_dim, int32_t unit,
                        int32_t out_shares, int32_t shares) {
   __shared__ float s_norm[GP * 2];
   __shared__ float s_acc[kJoinThreads / 32][32];
@@ -817,9 +814,11 @@ __global__ void __launch_bounds__(kJoinThreads)
   const int G = p.n_heads / p.n_kv;
   pdl_wait();
   pdl_launch_dependents();
+  const bool weights = p.weight_ptrs != nullptr;
   int32_t n = clamped_rows(p.n_pos, b, p.max_n_pos, p.status);
-  float* wts = p.weight_ptrs[b];
-  if (!usable_weights(wts, p.status) || !usable_ptrs(p.k_ptrs[b], p.v_ptrs[b], p.status)) n = 0;
+  float* wts = weights ? p.weight_ptrs[b] : nullptr;
+  if (weights && !usable_weights(wts, p.status)) n = 0;
+  if (!usable_ptrs(p.k_ptrs[b], p.v_ptrs[b], p.status)) n = 0;
   const int64_t row0 = (int64_t)share * kJoinRows;
   if (share < 0 && n == 0) {  // no rows: zeros
     if (tid < 32)
@@ -827,7 +826,9 @@ __global__ void __launch_bounds__(kJoinThreads)
     return;
   }
   if (row0 >= n) return;
-  const int32_t S = (int32_t)(((int64_t)n + p.part_rows - 1) / p.part_rows);  // parts with rows
+  // parts with rows (of a list: all, some perhaps without)
+  const int64_t part_rows = (int64_t)p.part_units * unit;
+  const int32_t S = weights ? (int32_t)((n + part_rows - 1) / part_rows) : p.S;
   const float2* ml = p.part_ml + (int64_t)item * G * p.S;
 
   constexpr int kPer = kJoinRows / kJoinThreads;
@@ -865,7 +866,7 @@ __global__ void __launch_bounds__(kJoinThreads)
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) {
       s_norm[warp * 2] = ref;
-      s_norm[warp * 2 + 1] = 1.0f / sum;
+      s_norm[warp * 2 + 1] = sum == 0.f ? 0.f : 1.0f / sum;  // no row listed: zeros
     }
   }
   __syncthreads();
@@ -916,6 +917,18 @@ int32_t part_rows_for(int32_t batch, int32_t n_kv, int64_t max_rows, int unit,
   int64_t rows = (max_rows * items + ctas - 1) / ctas;
   rows = std::max(least, (rows + step - 1) / step * step);
   return max_rows > rows ? (int32_t)rows : 0;
+}
+
+// The same for listed blocks: a cluster does it, unless so few lists are so long
+// that a cluster's warps (of 16 wide CTAs up to 7 lists, else of 16 slim ones) have
+// more than 4 units each while most of the device is idle.  One FP16 sequence of 8 kv
+// heads: 4096 rows 12.1 us by clusters and 11.8 by parts, 8192 16.4 and 14.4, 12,800
+// 21.2 and 16.3; of 4 kv heads: 4160 rows 9.2 and 12.0, 8192 11.3 and 11.8.  FP32, 8 kv
+// heads: 6400 rows 25.4 and 17.4.
+int64_t list_part_rows_for(int64_t items, int64_t rows, int unit, const DeviceInfo& dev) {
+  const int64_t step = 4 * unit, full = 3 * (int64_t)dev.sms;
+  if (items * 32 > full || rows <= 4 * (items < 8 ? 128 : 64) * (int64_t)unit) return 0;
+  return std::max(2 * step, (rows * items / full + step - 1) / step * step);
 }
 
 // Floats between the heads' scores: a last unit stores its rows past the end too.
@@ -978,13 +991,15 @@ int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t strea
   const int64_t rows = BLOCKS ? (int64_t)r.n_sel * r.block_rows : (int64_t)r.max_n_pos;
   const int64_t units = (rows + U - 1) / U;
   const int64_t items = (int64_t)r.batch * r.n_kv;
-  if constexpr (!BLOCKS) {
-    p.score_pitch = score_pitch_for(r.max_n_pos);
-    p.part_rows = part_rows_for(r.batch, r.n_kv, r.max_n_pos, U, dev);
-    if (p.part_rows) {
-      const int64_t parts = ((int64_t)r.max_n_pos + p.part_rows - 1) / p.part_rows;
+  if (!BLOCKS) p.score_pitch = score_pitch_for(r.max_n_pos);
+  {
+    const int64_t part_rows = BLOCKS ? list_part_rows_for(items, rows, U, dev)
+                                     : part_rows_for(r.batch, r.n_kv, rows, U, dev);
+    if (part_rows) {
+      p.part_units = (int32_t)(part_rows / U);
+      const int64_t parts = (rows + part_rows - 1) / part_rows;
       const int32_t outs = (r.n_heads / r.n_kv) * HD / 32;
-      const int64_t shares = ((int64_t)r.max_n_pos + kJoinRows - 1) / kJoinRows + outs;
+      const int64_t shares = (BLOCKS ? 0 : (rows + kJoinRows - 1) / kJoinRows) + outs;
       if (items * parts > INT32_MAX || items * shares > INT32_MAX) {
         *err = "batch * n_kv_heads * max_n_pos too large";
         return GLA_ERR_NOT_SUPPORTED;
@@ -996,7 +1011,7 @@ int launch_one(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t strea
       if (rc != GLA_OK) return rc;
       static ClusterKernel ck;
       return launch_clusters(attend_join_kernel, (unsigned)(items * shares), kJoinThreads, 0, 1,
-                             ck, stream, "attention join", err, p, (int32_t)HD, outs,
+                             ck, stream, "attention join", err, p, (int32_t)HD, U, outs,
                              (int32_t)shares);
     }
   }
@@ -1020,12 +1035,15 @@ int by_type(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream, 
 
 }  // namespace
 
-size_t attend_score_floats(const AttendRequest& r, const DeviceInfo& dev) {
+size_t attend_workspace_floats(const AttendRequest& r, const DeviceInfo& dev) {
   const int unit = r.dtype == GLA_DTYPE_F16 ? unit_rows<__half, 64>() : unit_rows<float, 64>();
-  const int64_t rows = part_rows_for(r.batch, r.n_kv, r.max_n_pos, unit, dev);
-  const int64_t parts = rows ? ((int64_t)r.max_n_pos + rows - 1) / rows : 0;
-  return (size_t)r.batch * r.n_heads *
-         (size_t)(score_pitch_for(r.max_n_pos) + parts * (r.head_dim + 2));
+  const int64_t rows = r.block_ids ? (int64_t)r.n_sel * r.block_rows : (int64_t)r.max_n_pos;
+  const int64_t part = r.block_ids
+                           ? list_part_rows_for((int64_t)r.batch * r.n_kv, rows, unit, dev)
+                           : part_rows_for(r.batch, r.n_kv, rows, unit, dev);
+  const int64_t parts = part ? (rows + part - 1) / part : 0;
+  const int64_t pitch = r.block_ids ? 0 : score_pitch_for(rows);
+  return (size_t)r.batch * r.n_heads * (size_t)(pitch + parts * (r.head_dim + 2));
 }
 
 int launch_attend(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,

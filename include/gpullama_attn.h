@@ -504,9 +504,10 @@ int32_t gla_rope_append_f32(gla_ctx* ctx, float* q, float* k, const float* v, fl
  *  - block_rows (16, 32, 64 or 128): block j is rows [j*block_rows, (j+1)*block_rows).
  *  - Results do not depend on timing: two calls on the same input give the
  *    same bits.
- *  - Calls can be captured in a CUDA graph; gla_decode_weights_* uses a context
- *    workspace that must have grown before (run its largest call once), so
- *    graphs of one context that hold it must not run at the same time. */
+ *  - Calls can be captured in a CUDA graph; gla_decode_weights_* and long lists of
+ *    gla_decode_blocks_* use a context workspace that must have grown before (run
+ *    the largest call once), so graphs of one context that hold them must not run at
+ *    the same time. */
 
 /* bounds: [n_blocks][n_kv_heads][2][head_dim] a sequence: the smallest (0) and the
  * largest (1) key of each channel over the rows t < n_pos of a block.  Exact; a NaN
@@ -575,7 +576,9 @@ int32_t gla_block_select_f16kv(gla_ctx* ctx, const float* q, const uint16_t* con
  * batch entry b attends only to the rows below n_pos[b] of the blocks block_ids[b][g][0
  * .. n_sel).  Negative ids and ids of blocks past the last row name no rows; a block
  * listed twice counts twice; no row at all gives zeros.  n_sel * block_rows < 2^31.
- * Batch entries may share caches (the queries of a prompt chunk). */
+ * Batch entries may share caches (the queries of a prompt chunk).  Long lists of a
+ * few sequences use the context workspace of gla_decode_weights_* (at most 2 MiB of
+ * it), grown on first use. */
 int32_t gla_decode_blocks_f32kv(gla_ctx* ctx, const float* q, const float* const* k_ptrs,
                                 const float* const* v_ptrs, const int32_t* n_pos,
                                 const int32_t* block_ids, int32_t n_sel, float* xb, int32_t batch,

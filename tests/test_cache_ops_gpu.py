@@ -302,7 +302,8 @@ def random_ids(g, lens, n_kv, br, n_sel):
 @pytest.mark.parametrize("t", TYPES)
 @pytest.mark.parametrize("nh,n_kv,hd", HEADS)
 @pytest.mark.parametrize("br,lens,n_sel", [(16, [1, 0, 333, 16, 47], 9), (64, [5000, 129], 24),
-                                           (128, [700], 3), (32, [20000], 200)])
+                                           (128, [700], 3), (32, [20000], 200),
+                                           (128, [0, 20000, 5], 150), (128, [19300], 140)])
 def test_decode_blocks_is_attention_over_the_listed_rows(gla_ctx, t, nh, n_kv, hd, br, lens, n_sel):
     g, pad = rng(8, nh, hd, br), 8
     k, v = caches(g, lens, n_kv, hd, t, pad_cols=pad), caches(g, lens, n_kv, hd, t, pad_cols=pad)
@@ -656,6 +657,43 @@ def test_a_served_batch_from_prompt_to_evicted_sparse_decode(gla_ctx, t):
         del graph
     stream.synchronize()
     ctx.close()
+
+
+def test_a_captured_long_list_needs_its_workspace(gla_ctx):
+    """Long lists of few heads are cut into parts in the context workspace."""
+    g, nh, n_kv, hd, br, n_sel = rng(26), 8, 2, 64, 128, 160
+    n = n_sel * br
+    k, v = caches(g, [n], n_kv, hd, "f16"), caches(g, [n], n_kv, hd, "f16")
+    q, xb = normal(g, 1, nh, hd), torch.empty(1, nh, hd, device="cuda")
+    ids = torch.arange(n_sel, dtype=torch.int32, device="cuda").repeat(1, n_kv, 1).contiguous()
+    kp, vp, np_ = ptrs(k), ptrs(v), i32([n])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    ctx = gla.Context(0, stream.cuda_stream)
+    call = lambda: ctx.decode_blocks(q, kp, vp, np_, ids, n_sel, xb, 1, nh, n_kv, hd, br, f16_cache=True)  # noqa: E731
+    with torch.cuda.stream(stream):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(gla.GlaError, match="must grow"):
+            with torch.cuda.graph(graph, stream=stream):
+                call()
+        call()
+        want = xb.clone()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call()
+        for _ in range(3):
+            xb.zero_()
+            graph.replay()
+            assert torch.equal(xb, want)
+        del graph
+    stream.synchronize()
+    assert ctx.device_status() == 0
+    ctx.close()
+    for h in range(n_kv):
+        qh, kk, vv = q[0, 4 * h:4 * h + 4], rows_of(k[0], n, n_kv, hd)[:, h], rows_of(v[0], n, n_kv, hd)[:, h]
+        got, (o, _) = want[0, 4 * h:4 * h + 4], attend64(qh, kk, vv, 1 / 8)
+        assert float((got.double() - o).abs().max()) <= attention_bound(qh, kk, vv, 1 / 8)[0]
 
 
 def test_a_captured_weights_call_survives_a_larger_one(gla_ctx):
