@@ -13,10 +13,14 @@
 // each kept row read and written once): to another cache, every (row, 16-byte chunk)
 // by itself; in place, in rounds (below).
 //
-// Measured on one B200: 4096 rows of 8 kv heads to 1024, FP32, 10.3 us (two launches,
-// each a chain of loads); 16 sequences of up to 32,768 FP16 rows to 4096 110 us, 21
+// Calls of few kv heads do both in one launch (evict_small_kernel).
+//
+// Measured on one B200: 4096 rows of 8 kv heads to 1024, FP32, 8.4 us (a chain of loads
+// and passes); 16 sequences of up to 32,768 FP16 rows to 4096 110 us, 21
 // the selection (the longest sequence's walks) and 87 the copy (6.2 TB/s read and
 // written).
+#include <algorithm>
+
 #include "cache_ops.cuh"
 
 namespace gla {
@@ -25,6 +29,34 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kMoveThreads = 256;
+
+// Selects the `pick` largest of the CTA's weights mine[0 .. count) (of a cluster's,
+// if S > 1) and hands their indices to emit(index, position), ascending.  Keys are
+// staged in s_key if they fit, else the weights are read again a pass.
+template <class Emit>
+__device__ __forceinline__ void select_weights(SelectScratch& sh, uint32_t* s_key, int S, int rank,
+                                               const float* mine, int32_t count, int32_t pick,
+                                               bool fits, Emit emit) {
+  uint32_t kmin = ~0u, kmax = 0;
+#pragma unroll 8
+  for (int32_t i = threadIdx.x; i < count; i += kSelThreads) {
+    const uint32_t k = order_key(__ldcg(mine + i));
+    if (fits) s_key[i] = k;
+    kmin = min(kmin, k);
+    kmax = max(kmax, k);
+  }
+  if (fits) fill_up_keys(s_key, count);
+  key_range<kSelThreads>(sh, S, &kmin, &kmax);  // (a barrier: the keys are staged)
+  auto select = [&](auto key) {
+    const Threshold<uint32_t> th = find_threshold<kSelThreads, uint32_t>(
+        sh, S, count, (uint32_t)pick, kmin, kmax, key);
+    emit_chosen<kSelThreads, uint32_t>(sh, S, rank, count, th, key, emit);
+  };
+  if (fits)
+    select(SharedKeys{s_key});
+  else
+    select(keys_by([&](int32_t i) { return order_key(__ldcg(mine + i)); }));
+}
 
 __global__ void __launch_bounds__(kSelThreads)
     evict_select_kernel(const float* const* __restrict__ weight_ptrs, int64_t weight_stride,
@@ -54,29 +86,81 @@ __global__ void __launch_bounds__(kSelThreads)
   if (pick == 0) return;
   int32_t lo, hi;
   share_of(older, S, rank, &lo, &hi);
-  const float* mine = w + (int64_t)g * weight_stride + lo;
-  const bool fits = (older + S - 1) / S <= key_cap;  // (not so past 16 CTAs' shared memory)
-  uint32_t kmin = ~0u, kmax = 0;
-#pragma unroll 8
-  for (int32_t i = tid; i < hi - lo; i += kSelThreads) {
-    const uint32_t k = order_key(__ldcg(mine + i));
-    if (fits) s_key[i] = k;
-    kmin = min(kmin, k);
-    kmax = max(kmax, k);
-  }
-  if (fits) fill_up_keys(s_key, hi - lo);
-  key_range<kSelThreads>(sh, S, &kmin, &kmax);  // (a barrier: the keys are staged)
-  auto select = [&](auto key) {
-    const Threshold<uint32_t> th = find_threshold<kSelThreads, uint32_t>(
-        sh, S, hi - lo, (uint32_t)pick, kmin, kmax, key);
-    emit_chosen<kSelThreads, uint32_t>(sh, S, rank, hi - lo, th, key,
-                                       [&](int32_t i, uint32_t at) { out[at] = lo + i; });
-  };
   // the ranks' shares differ by rounding alone, and every rank takes the same way
-  if (fits)
-    select(SharedKeys{s_key});
-  else
-    select(keys_by([&](int32_t i) { return order_key(__ldcg(mine + i)); }));
+  const bool fits = (older + S - 1) / S <= key_cap;  // (not so past 16 CTAs' shared memory)
+  select_weights(sh, s_key, S, rank, w + (int64_t)g * weight_stride + lo, hi - lo, pick, fits,
+                 [&](int32_t i, uint32_t at) { out[at] = lo + i; });
+}
+
+// Selection and copy to another cache in one launch, for calls of few kv heads:
+// `parts` CTAs of an item each select all of it (the weights are read from L2) and
+// copy a share of the kept rows, which saves the second launch and its first loads
+// (4096 FP32 rows of 8 kv heads to 1024: 8.4 us, in two launches 10.3).
+template <int kChunks, int kPer, class T>
+__global__ void __launch_bounds__(kSelThreads)
+    evict_small_kernel(T* const* __restrict__ k_ptrs, T* const* __restrict__ v_ptrs,
+                       float* const* __restrict__ weight_ptrs, int64_t weight_stride,
+                       T* const* __restrict__ k_out_ptrs, T* const* __restrict__ v_out_ptrs,
+                       float* const* __restrict__ weight_out_ptrs, int64_t weight_out_stride,
+                       const int32_t* __restrict__ n_pos, int32_t max_n_pos, int32_t n_keep,
+                       int32_t n_recent, int32_t* __restrict__ kept, int32_t n_kv,
+                       int64_t kv_stride, int32_t parts, int32_t key_words,
+                       int32_t* __restrict__ status) {
+  extern __shared__ __align__(16) uint32_t s_key[];  // keys, then the list of kept rows
+  __shared__ SelectScratch sh;
+  pdl_wait();
+  const int tid = threadIdx.x;
+  const int item = (int)(blockIdx.x / (unsigned)parts), part = (int)(blockIdx.x % (unsigned)parts);
+  const int b = item / n_kv, g = item - b * n_kv;
+  const T* k = k_ptrs[b];
+  const T* v = v_ptrs[b];
+  const float* w = weight_ptrs[b];
+  T* ko = k_out_ptrs[b];
+  T* vo = v_out_ptrs[b];
+  float* wo = weight_out_ptrs[b];
+  int32_t n = clamped_rows(n_pos, b, max_n_pos, status);
+  bool move = true;
+  if (!usable_weights(w, status)) {
+    n = 0;
+  } else if (!usable_ptrs(k, v, status) || !usable_ptrs(ko, vo, status) ||
+             !usable_weights(wo, status)) {
+    move = false;
+  } else if (k == ko || v == vo || w == wo) {  // another order of moves is needed in place
+    if (tid == 0) atomicCAS(status, 0, GLA_ERR_INVALID_ARG);
+    move = false;
+  }
+  int32_t* list = reinterpret_cast<int32_t*>(s_key) + key_words;
+  const int32_t m = min(n, n_keep);
+  w += (int64_t)g * weight_stride;
+  if (n > n_keep) {
+    const int32_t older = n - n_recent, pick = n_keep - n_recent;
+    for (int32_t i = tid; i < n_recent; i += kSelThreads) list[pick + i] = older + i;
+    if (pick > 0)
+      select_weights(sh, s_key, 1, 0, w, older, pick, true,
+                     [&](int32_t i, uint32_t at) { list[at] = i; });
+  } else {
+    for (int32_t i = tid; i < m; i += kSelThreads) list[i] = i;
+  }
+  __syncthreads();
+  if (part == 0)
+    for (int32_t i = tid; i < n_keep; i += kSelThreads)
+      kept[(int64_t)item * n_keep + i] = i < m ? list[i] : -1;
+  if (!move) return;
+  const int32_t r0 = (int32_t)((int64_t)m * part / parts);
+  const int32_t r1 = (int32_t)((int64_t)m * (part + 1) / parts);
+  const int64_t col = (int64_t)g * kChunks * kPer;
+#pragma unroll 2
+  for (int32_t i = tid; i < (r1 - r0) * kChunks; i += kSelThreads) {
+    const int32_t r = r0 + i / kChunks, c = i % kChunks;
+    const int64_t src = (int64_t)list[r] * kv_stride + col + c * kPer;
+    const int64_t dst = (int64_t)r * kv_stride + col + c * kPer;
+    const float4 xk = __ldcg(reinterpret_cast<const float4*>(k + src));
+    const float4 xv = __ldcg(reinterpret_cast<const float4*>(v + src));
+    *reinterpret_cast<float4*>(ko + dst) = xk;
+    *reinterpret_cast<float4*>(vo + dst) = xv;
+  }
+  for (int32_t r = r0 + tid; r < r1; r += kSelThreads)
+    wo[(int64_t)g * weight_out_stride + r] = w[list[r]];
 }
 
 // Kept rows of one kv head to another cache: thread = (row, 16-byte chunk).
@@ -239,6 +323,51 @@ int launch_pdl(void (*kern)(Params...), unsigned grid, int threads, cudaStream_t
   return GLA_OK;
 }
 
+// CTAs of an item when one launch does it all, 0 when two do: the CTAs have to
+// hold all keys and the list, must not make a second wave, and where they leave half
+// of the device idle, the copy must be short (measured, one launch against two: 64 kv
+// heads of 1000 to 8192 FP16 rows to 2048 31 and 33 us; 4 kv heads of 32,768 FP32
+// rows to 16,384 on 64 CTAs 51 and 46).
+int small_parts(const EvictRequest& r, const DeviceInfo& dev, int32_t* key_words) {
+  const int64_t items = (int64_t)r.batch * r.n_kv;
+  const int64_t keys = ((int64_t)r.max_n_pos + 3) / 4 * 4;
+  const int64_t most = std::min(r.n_keep, r.max_n_pos);
+  if (!r.k_out_ptrs || items * 2 > dev.sms || r.max_n_pos > 32768 ||
+      (keys + most) * 4 > dev.smem_optin - 12 * 1024)
+    return 0;
+  *key_words = (int32_t)keys;
+  const int64_t parts = std::max<int64_t>(1, std::min({(int64_t)16, dev.sms / items, (most + 31) / 32}));
+  const int64_t bytes = most * 2 * r.head_dim * (r.dtype == GLA_DTYPE_F16 ? 2 : 4);
+  return 2 * items * parts < dev.sms && bytes > parts * 128 * 1024 ? 0 : (int)parts;
+}
+
+template <class T, int HD>
+int launch_small(const EvictRequest& r, int parts, int32_t key_words, cudaStream_t stream,
+                 std::string* err) {
+  static ClusterKernel ck;
+  constexpr int kPer = 16 / sizeof(T);
+  const int64_t items = (int64_t)r.batch * r.n_kv;
+  const size_t smem = ((size_t)key_words + std::min(r.n_keep, r.max_n_pos)) * 4;
+  return launch_clusters(evict_small_kernel<HD / kPer, kPer, T>, (unsigned)(items * parts),
+                         kSelThreads, smem, 1, ck, stream, "evict",
+                         err, reinterpret_cast<T* const*>(r.k_ptrs),
+                         reinterpret_cast<T* const*>(r.v_ptrs), r.weight_ptrs, r.weight_stride,
+                         reinterpret_cast<T* const*>(r.k_out_ptrs),
+                         reinterpret_cast<T* const*>(r.v_out_ptrs), r.weight_out_ptrs,
+                         r.weight_out_stride, r.n_pos, r.max_n_pos, r.n_keep, r.n_recent, r.kept,
+                         r.n_kv, r.kv_stride, (int32_t)parts, key_words, r.status);
+}
+
+template <class T>
+int small_dim(const EvictRequest& r, int parts, int32_t key_words, cudaStream_t stream,
+              std::string* err) {
+  switch (r.head_dim) {
+    case 64: return launch_small<T, 64>(r, parts, key_words, stream, err);
+    case 96: return launch_small<T, 96>(r, parts, key_words, stream, err);
+    default: return launch_small<T, 128>(r, parts, key_words, stream, err);
+  }
+}
+
 template <class T, int HD>
 int launch_move(const EvictRequest& r, cudaStream_t stream, std::string* err) {
   constexpr int kPer = 16 / sizeof(T);
@@ -285,6 +414,10 @@ int move_dim(const EvictRequest& r, cudaStream_t stream, std::string* err) {
 
 int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stream,
                  std::string* err) {
+  int32_t key_words = 0;
+  if (const int parts = small_parts(r, dev, &key_words))
+    return r.dtype == GLA_DTYPE_F16 ? small_dim<__half>(r, parts, key_words, stream, err)
+                                    : small_dim<float>(r, parts, key_words, stream, err);
   static ClusterKernel ck;
   const int64_t items = (int64_t)r.batch * r.n_kv;
   // One CTA a kv head up to 32,768 weights: each of the passes of a cluster costs it

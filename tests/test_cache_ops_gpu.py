@@ -490,7 +490,8 @@ def kept64(w, n, keep, recent):
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("n_kv,hd,lens,keep,recent", [
     (8, 128, [700, 64, 65, 0, 3], 64, 16), (2, 64, [5000, 4999], 1200, 0), (3, 96, [2000], 1, 1),
-    (1, 64, [40000], 9000, 9000), (4, 96, [1300, 1300], 1299, 5), (2, 128, [30], 50, 7)])
+    (1, 64, [40000], 9000, 9000), (4, 96, [1300, 1300], 1299, 5), (2, 128, [30], 50, 7),
+    (2, 64, [33, 700, 20, 0, 21] * 16, 20, 3), (16, 96, [900] * 10, 300, 40)])
 def test_evict_keeps_the_heaviest_rows(gla_ctx, t, in_place, n_kv, hd, lens, keep, recent):
     g, pad, top = rng(14, n_kv, hd, keep), 8, max(lens)
     batch, stride = len(lens), n_kv * hd + pad
