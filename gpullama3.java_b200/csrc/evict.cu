@@ -11,14 +11,15 @@
 // the weights with the radix selection of cache_ops.cuh, its keys in shared memory,
 // and writes the ascending list.  The rows then move in a second kernel (HBM-bound,
 // each kept row read and written once): to another cache, every (row, 16-byte chunk)
-// by itself; in place, in rounds (below).
+// by itself; in place, a cluster a (sequence, kv head), in rounds (evict_compact_kernel).
 //
 // Calls of few kv heads do both in one launch (evict_small_kernel).
 //
 // Measured on one B200: 4096 rows of 8 kv heads to 1024, FP32, 8.4 us (a chain of loads
 // and passes); 16 sequences of up to 32,768 FP16 rows to 4096 110 us, 21
 // the selection (the longest sequence's walks) and 87 the copy (6.2 TB/s read and
-// written).
+// written); the same in place 151 us (16 of exactly 32,768 rows; one CTA a head and
+// 64 columns of K or V: 209).
 #include <algorithm>
 
 #include "cache_ops.cuh"
@@ -223,83 +224,97 @@ __global__ void __launch_bounds__(kMoveThreads)
     wo[(int64_t)g * weight_out_stride + row0 + r] = w[(int64_t)g * weight_stride + list[row0 + r]];
 }
 
-// In place.  One CTA moves a column slice of 64 bytes (4 chunks) of K or of V
-// of one (sequence, kv head), or its weights, so slices never touch each
-// other's bytes.  Rows move in rounds of kRound list entries: all loads of a
-// round, a barrier, its stores.  A kept row's source is never below its
-// destination (list[i] >= i, ascending), so the stores of round r, to rows
-// below (r + 1) kRound, can only hit sources of rounds <= r, which are all
-// loaded; the loads of round r + 1 may therefore be in flight meanwhile.
-template <int kSlices, int kPer, class T>
-__global__ void __launch_bounds__(kMoveThreads)
+// In place.  A cluster of S CTAs moves the rows of K and V of one (sequence, kv
+// head), and its weights, in rounds of as many (row, 16-byte chunk) pairs as its
+// threads take kUnroll each: all loads of a round, a cluster barrier, its stores.
+// A kept row's source is never below its destination (list[i] >= i, ascending), so
+// the stores of round r, to rows below the next round's first, can only hit sources
+// of rounds <= r, which are all loaded; the loads of round r + 1 may therefore be in
+// flight meanwhile, and the list entries of round r + 2 (which hides both their
+// latency: 16 x 32,768 FP16 rows to 4096, 178 us with the entries read at their load).
+template <int kChunks, int kPer, class T>
+__global__ void __launch_bounds__(kMoveThreads, 2)
     evict_compact_kernel(T* const* __restrict__ k_ptrs, T* const* __restrict__ v_ptrs,
                          float* const* __restrict__ weight_ptrs, int64_t weight_stride,
                          const int32_t* __restrict__ n_pos, int32_t max_n_pos, int32_t n_keep,
-                         const int32_t* __restrict__ kept, int32_t n_kv, int64_t kv_stride,
+                         const int32_t* __restrict__ kept, int32_t n_kv, int64_t kv_stride, int S,
                          int32_t* __restrict__ status) {
   constexpr int kUnroll = 8;
-  constexpr int kStep = kMoveThreads / 4;       // rows side by side
-  constexpr int kRound = kStep * kUnroll;
-  constexpr int kParts = 2 * kSlices + 1;       // K slices, V slices, weights
+  constexpr int kRow = 2 * kChunks;  // chunks of a row: K's, then V's
   pdl_wait();
-  const int tid = threadIdx.x;
-  const int item = (int)(blockIdx.x / kParts), part = (int)(blockIdx.x % kParts);
+  const int rank = S > 1 ? (int)(blockIdx.x % (unsigned)S) : 0;
+  const int item = (int)(blockIdx.x / (unsigned)S);
   const int b = item / n_kv, g = item - b * n_kv;
   const int32_t n = clamped_rows(n_pos, b, max_n_pos, status);
-  if (n <= n_keep) return;
+  if (n <= n_keep) return;  // every CTA of the cluster takes these ways
   T* k = k_ptrs[b];
   T* v = v_ptrs[b];
   float* w = weight_ptrs[b];
   if (!usable_ptrs(k, v, status) || !usable_weights(w, status)) return;
   const int32_t* list = kept + (int64_t)item * n_keep;
-  if (part == kParts - 1) {
-    w += (int64_t)g * weight_stride;
-    constexpr int kWr = kMoveThreads * kUnroll;
-    for (int32_t i0 = 0; i0 < n_keep; i0 += kWr) {
-      float x[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int32_t i = i0 + u * kMoveThreads + tid;
-        if (i < n_keep) x[u] = __ldcg(w + list[i]);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int32_t i = i0 + u * kMoveThreads + tid;
-        if (i < n_keep) w[i] = x[u];
-      }
-    }
-    // the rows behind have no weight yet: a token appended there starts at zero
-    __syncthreads();
-    for (int32_t i = n_keep + tid; i < n; i += kMoveThreads) w[i] = 0.f;
-    return;
-  }
-  T* base = (part < kSlices ? k : v) + (int64_t)g * kSlices * 4 * kPer +
-            (part % kSlices) * 4 * kPer + (tid & 3) * kPer;
-  const int r0 = tid >> 2;
+  const int me = rank * kMoveThreads + (int)threadIdx.x, all = S * kMoveThreads;
+  k += (int64_t)g * kChunks * kPer;
+  v += (int64_t)g * kChunks * kPer;
+  w += (int64_t)g * weight_stride;
+
+  const int32_t round = all * kUnroll / kRow;  // rows
   float4 cur[kUnroll], nxt[kUnroll];
-  int32_t from[kUnroll], from_next[kUnroll];
-  auto load = [&](int32_t i0, float4 (&x)[kUnroll], int32_t (&src)[kUnroll]) {
+  // sources of the round at work, of the next (its rows under way), of the one after
+  int32_t from[kUnroll], from_next[kUnroll], from_then[kUnroll];
+  // chunk u of this thread: row i0 + e / kRow of the round, chunk e % kRow
+  auto at = [&](int32_t row, int c) {
+    return (c < kChunks ? k : v) + (int64_t)row * kv_stride + (c % kChunks) * kPer;
+  };
+  auto sources = [&](int32_t i0, int32_t (&src)[kUnroll]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int32_t i = i0 + u * kStep + r0;
-      src[u] = i < n_keep ? list[i] : i;
-      // a row that stays needs no move
-      if (src[u] != i) x[u] = __ldcg(reinterpret_cast<const float4*>(base + (int64_t)src[u] * kv_stride));
+      const int r = (u * all + me) / kRow;
+      const int32_t i = i0 + r;
+      src[u] = r < round && i < n_keep ? list[i] : i;  // (nothing to move)
     }
   };
-  load(0, cur, from);
-  for (int32_t i0 = 0; i0 < n_keep; i0 += kRound) {
-    __syncthreads();  // every load of this round is done
-    if (i0 + kRound < n_keep) load(i0 + kRound, nxt, from_next);
+  auto load = [&](int32_t i0, float4 (&x)[kUnroll], const int32_t (&src)[kUnroll]) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int32_t i = i0 + u * kStep + r0;
-      if (from[u] != i) *reinterpret_cast<float4*>(base + (int64_t)i * kv_stride) = cur[u];
+      const int e = u * all + me;
+      // a row that stays needs no move
+      if (src[u] != i0 + e / kRow) x[u] = __ldcg(reinterpret_cast<const float4*>(at(src[u], e % kRow)));
+    }
+  };
+  sources(0, from);
+  sources(round, from_next);
+  load(0, cur, from);
+  for (int32_t i0 = 0; i0 < n_keep; i0 += round) {
+    cluster_barrier(S);  // every load of this round is done
+    load(i0 + round, nxt, from_next);
+    sources(i0 + 2 * round, from_then);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int e = u * all + me;
+      const int32_t i = i0 + e / kRow;
+      if (from[u] != i) *reinterpret_cast<float4*>(at(i, e % kRow)) = cur[u];
       cur[u] = nxt[u];
       from[u] = from_next[u];
+      from_next[u] = from_then[u];
     }
   }
+  for (int32_t i0 = 0; i0 < n_keep; i0 += all * kUnroll) {
+    float x[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int32_t i = i0 + u * all + me;
+      if (i < n_keep) x[u] = __ldcg(w + list[i]);
+    }
+    cluster_barrier(S);
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int32_t i = i0 + u * all + me;
+      if (i < n_keep) w[i] = x[u];
+    }
+  }
+  // the rows behind have no weight yet: a token appended there starts at zero (every
+  // source is loaded: the last round's barrier)
+  for (int32_t i = n_keep + me; i < n; i += all) w[i] = 0.f;
 }
 
 template <class... Params, class... Args>
@@ -369,7 +384,8 @@ int small_dim(const EvictRequest& r, int parts, int32_t key_words, cudaStream_t 
 }
 
 template <class T, int HD>
-int launch_move(const EvictRequest& r, cudaStream_t stream, std::string* err) {
+int launch_move(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stream,
+                std::string* err) {
   constexpr int kPer = 16 / sizeof(T);
   constexpr int kChunks = HD / kPer;
   const int64_t items = (int64_t)r.batch * r.n_kv;
@@ -389,24 +405,33 @@ int launch_move(const EvictRequest& r, cudaStream_t stream, std::string* err) {
                       r.weight_out_stride, r.n_pos, r.max_n_pos, r.n_keep,
                       (const int32_t*)r.kept, r.n_kv, r.kv_stride, (int32_t)parts, r.status);
   }
-  constexpr int kSlices = kChunks / 4;
-  const int64_t grid = items * (2 * kSlices + 1);
-  if (grid > INT32_MAX) {
+  // CTAs of an item's cluster: as many as the device holds at once (two an SM), while
+  // a round is not more than half of the rows
+  static ClusterKernel ck;
+  auto kern = evict_compact_kernel<kChunks, kPer, T>;
+  int S = 1;
+  while (S < 16 && items * S * 2 <= 2 * dev.sms &&
+         (int64_t)2 * S * kMoveThreads * 8 / (2 * kChunks) * 2 <= r.n_keep &&
+         items <= clusters_held(kern, ck, kMoveThreads, 0, 2 * S, dev))
+    S *= 2;
+  if (items * S > INT32_MAX) {
     *err = "batch * n_kv_heads too large";
     return GLA_ERR_NOT_SUPPORTED;
   }
-  return launch_pdl(evict_compact_kernel<kSlices, kPer, T>, (unsigned)grid, kMoveThreads, stream,
-                    "evict compaction", err, reinterpret_cast<T* const*>(r.k_ptrs),
-                    reinterpret_cast<T* const*>(r.v_ptrs), r.weight_ptrs, r.weight_stride, r.n_pos,
-                    r.max_n_pos, r.n_keep, (const int32_t*)r.kept, r.n_kv, r.kv_stride, r.status);
+  return launch_clusters(kern, (unsigned)(items * S), kMoveThreads, 0, S, ck, stream,
+                         "evict compaction", err, reinterpret_cast<T* const*>(r.k_ptrs),
+                         reinterpret_cast<T* const*>(r.v_ptrs), r.weight_ptrs, r.weight_stride,
+                         r.n_pos, r.max_n_pos, r.n_keep, (const int32_t*)r.kept, r.n_kv,
+                         r.kv_stride, S, r.status);
 }
 
 template <class T>
-int move_dim(const EvictRequest& r, cudaStream_t stream, std::string* err) {
+int move_dim(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stream,
+             std::string* err) {
   switch (r.head_dim) {
-    case 64: return launch_move<T, 64>(r, stream, err);
-    case 96: return launch_move<T, 96>(r, stream, err);
-    default: return launch_move<T, 128>(r, stream, err);
+    case 64: return launch_move<T, 64>(r, dev, stream, err);
+    case 96: return launch_move<T, 96>(r, dev, stream, err);
+    default: return launch_move<T, 128>(r, dev, stream, err);
   }
 }
 
@@ -439,8 +464,8 @@ int launch_evict(const EvictRequest& r, const DeviceInfo& dev, cudaStream_t stre
                            (const float* const*)r.weight_ptrs, r.weight_stride, r.n_pos,
                            r.max_n_pos, r.n_keep, r.n_recent, r.kept, r.n_kv, S, key_cap, r.status);
   if (rc != GLA_OK) return rc;
-  return r.dtype == GLA_DTYPE_F16 ? move_dim<__half>(r, stream, err)
-                                  : move_dim<float>(r, stream, err);
+  return r.dtype == GLA_DTYPE_F16 ? move_dim<__half>(r, dev, stream, err)
+                                  : move_dim<float>(r, dev, stream, err);
 }
 
 }  // namespace gla

@@ -13,8 +13,9 @@
 // in shared memory (cp.async, 16 bytes a lane, rows past the last one zero-filled
 // and never read) and keeps its own running maximum, sum and output: no block
 // barrier inside the stream.  The warps join in shared memory and the CTAs through
-// the cluster's shared memory, in a fixed order, so results do not depend on timing,
-// and listed blocks need no workspace, counter or second launch.  Rows in shared
+// the cluster's shared memory, in a fixed order, so results do not depend on timing.
+// Long lists of few kv heads are cut into parts, one CTA each, that a second kernel
+// joins (list_part_rows_for).  Rows in shared
 // memory are padded by 16 bytes: a row's pitch is an odd number of 16-byte chunks,
 // which keeps ldmatrix and the vector loads free of bank conflicts.  (One bulk copy
 // a row instead of 16 cp.async a lane: 320 us against 244 for 256 queries over
