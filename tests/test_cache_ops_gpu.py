@@ -541,6 +541,26 @@ def test_evict_keeps_the_heaviest_rows(gla_ctx, t, in_place, n_kv, hd, lens, kee
                 assert (wo[b][h, m:] == 3.0).all()
 
 
+@pytest.mark.parametrize("n,keep,recent", [(40_001, 30_000, 1), (100_003, 7000, 33), (900_005, 20_001, 2)])
+def test_evict_long_interleaved_sequences_in_place(gla_ctx, n, keep, recent):
+    """Selections over the CTAs of a cluster (the longest past their shared memory), with ties
+    over all of them; K and V are the two halves of one row."""
+    g, hd = rng(26, n), 64
+    kv = normal(g, n, 2 * hd).half()
+    k, v = kv[:, :hd], kv[:, hd:]
+    w = torch.exp(normal(g, 1, n))
+    w[0, ::2] = 1.0
+    kv0, w0 = kv.clone(), w.clone()
+    kept = torch.empty(1, 1, keep, dtype=torch.int32, device="cuda")
+    gla_ctx.kv_evict(ptrs([k]), ptrs([v]), ptrs([w]), n, i32([n]), n, keep, recent, kept, 1, 1, hd,
+                     kv_stride=2 * hd, f16_cache=True)
+    ok(gla_ctx)
+    rows = kept64(w0[0], n, keep, recent)
+    assert kept[0, 0].tolist() == rows
+    assert torch.equal(kv[:keep], kv0[rows]) and torch.equal(kv[keep:], kv0[keep:])
+    assert torch.equal(w[0, :keep], w0[0, rows]) and (w[0, keep:] == 0).all()
+
+
 def test_evict_to_the_same_cache_is_refused(gla_ctx):
     g = rng(15)
     k, v = caches(g, [50, 50], 2, 64, "f32"), caches(g, [50, 50], 2, 64, "f32")
