@@ -43,8 +43,8 @@
 //
 // Measured on one B200: listed blocks, 64 of 64 FP16 rows for 4 kv heads of 128
 // 8.6 us (latency: 131 KB an SM through 64 bytes a clock, then the joins); 256
-// queries over one cache of 32,768 rows, 32 blocks each, 212 us (2.1 GB through L2,
-// 10 TB/s); 64 separate FP16 caches 107 us, 5.0 TB/s.  Weights, 131,072 FP16 rows of
+// queries over one cache of 32,768 rows, 32 blocks each, 220 us (2.1 GB through L2,
+// 9.8 TB/s); 64 separate FP16 caches 105 us, 5.1 TB/s.  Weights, 131,072 FP16 rows of
 // 4 kv heads 60 us (4.6 TB/s with scores and weights).
 #include <cmath>
 
@@ -651,7 +651,7 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   // unit i of this warp is first + i * stride; its ring slot i % kStages.  A slot
   // is filled again as soon as it is read out, so while a warp waits for a unit the
   // ring's other units are under way too.
-  const int32_t mine = units > first ? (units - first - 1) / stride + 1 : 0;
+  int32_t mine = units > first ? (units - first - 1) / stride + 1 : 0;
   int32_t row_of[kStages];
   auto fetch = [&](int s, int32_t i, int32_t id) {
     row_of[s] = -1;
@@ -666,8 +666,24 @@ __global__ void __launch_bounds__(Cta<T, HD, WIDE>::kThreads, Cta<T, HD, WIDE>::
   for (int s = 0; s < kStages; ++s) fetch(s, s, id[s]);
   int32_t next_id = id[kStages];  // ids are loaded a step before the rows they name
   if (WIDE) cluster_arrive(S);
+  const int32_t tail_id = BLOCKS && p.n_sel - 32 + lane >= 0 ? __ldg(ids + p.n_sel - 32 + lane) : -1;
   Warp w;  // while the first units are under way
   w.template init<kWarps>(query, p.scale_log2, s_q, warp, lane);
+  // A list counts up to its last id that names rows: the short sequences of a batch
+  // leave much of theirs empty, and an empty unit too costs a warp a step (960 lists of
+  // up to 4 blocks of 64 rows in 64 slots: 45 us, in 4 slots 19).
+  if (BLOCKS && mine > kStages) {
+    int32_t used = 0;
+    for (int32_t end = p.n_sel; end > 0 && used == 0; end -= 32) {
+      const int32_t i = end - 32 + lane;
+      const int32_t last = end == p.n_sel ? tail_id : i < 0 ? -1 : __ldg(ids + i);
+      const unsigned named = __ballot_sync(
+          0xffffffffu, last >= 0 && ((int64_t)last << p.br_shift) < n);
+      if (named) used = end - __clz((int)named);
+    }
+    units = min(units, used << (p.br_shift - kShift));
+    mine = units > first ? (units - first - 1) / stride + 1 : 0;
+  }
   for (int32_t i0 = 0; i0 < mine; i0 += kStages) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) {

@@ -338,6 +338,39 @@ def test_decode_blocks_is_attention_over_the_listed_rows(gla_ctx, t, nh, n_kv, h
 
 
 @pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("batch,n_sel", [(1, 257), (40, 100)])
+def test_decode_blocks_over_lists_that_are_mostly_empty(gla_ctx, t, batch, n_sel):
+    """Named blocks anywhere in a long list, its other slots naming no rows."""
+    g, nh, n_kv, hd, br = rng(27, batch), 8, 4, 64, 64
+    lens = [1 + 173 * i % 700 for i in range(batch)]
+    k, v = caches(g, lens, n_kv, hd, t), caches(g, lens, n_kv, hd, t)
+    q = normal(g, batch, nh, hd)
+    ids = torch.full((batch, n_kv, n_sel), -1, dtype=torch.int32, device="cuda")
+    ids[:, :, 33::5] = 11  # no sequence has a block 11
+    at = [[], [0], [n_sel - 1], [1, n_sel - 33, n_sel - 32]]
+    for h in range(n_kv):
+        for s in at[h]:
+            ids[:, h, s] = s % 3
+    xb = torch.full((batch, nh, hd), float("nan"), device="cuda")
+    gla_ctx.decode_blocks(q, ptrs(k), ptrs(v), i32(lens), ids, n_sel, xb, batch, nh, n_kv, hd, br,
+                          f16_cache=t == "f16")
+    ok(gla_ctx)
+    scale = 1 / math.sqrt(hd)
+    for b, n in enumerate(lens):
+        kk, vv = rows_of(k[b], n, n_kv, hd), rows_of(v[b], n, n_kv, hd)
+        for h in range(n_kv):
+            rows = [r for j in ids[b, h].tolist() if j >= 0 for r in range(j * br, min(n, (j + 1) * br))]
+            got = xb[b, 2 * h:2 * h + 2]
+            if not rows:
+                assert (got == 0).all()
+                continue
+            x = torch.tensor(rows, dtype=torch.int64, device="cuda")
+            want, _ = attend64(q[b, 2 * h:2 * h + 2], kk[x, h], vv[x, h], scale)
+            tol, _ = attention_bound(q[b, 2 * h:2 * h + 2], kk[x, h], vv[x, h], scale)
+            assert float((got.double() - want).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("t", TYPES)
 def test_decode_blocks_listed_twice_and_shared_caches(gla_ctx, t):
     """A block listed twice counts twice; queries of one chunk share a cache, each with
     its own length and blocks."""
