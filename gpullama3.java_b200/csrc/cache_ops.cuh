@@ -376,7 +376,7 @@ __device__ __forceinline__ void emit_chosen(SelectScratch& sh, int S, int rank, 
   const bool fast = KeyFn::kQuads && th.whole;
   uint32_t above = 0, at = 0;
   if constexpr (KeyFn::kQuads) {
-    if (fast) {
+    if (fast && w_lo < w_hi) {  // (an empty share starts at n_local, inside a quad)
 #pragma unroll 4
       for (int32_t q = w_lo / 4 + lane; q < (w_hi + 3) / 4; q += 32) {
         const uint4 kv = key.quad(q);
