@@ -355,7 +355,10 @@ __device__ __forceinline__ Threshold<Key> find_threshold(SelectScratch& sh, int 
     need -= sh.found[1];
     whole = sh.found[2] == need;
     base += (Key)sh.found[0] << shift;
+    // the last digit's range ends at kmax: past the type's end it would hold the lowest
+    // keys too, the filling ones among them
     span = ((Key)1 << shift) - 1;
+    span = span < kmax - base ? span : kmax - base;
     if (whole || shift == 0) break;
     shift = shift > 8 ? shift - 8 : 0;
   }

@@ -73,3 +73,22 @@ def test_eviction_of_an_odd_batch_over_clusters(gla_ctx, t, in_place):
     lens = [2400 + i for i in range(1, 10)] + [1283, 3071 + 2048, 32_999]
     w = [torch.rand(n_kv, top, generator=g, device="cuda") for _ in lens]
     evict_and_check(gla_ctx, g, t, in_place, n_kv, hd, lens, w, 2399, 0, top)
+
+
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("in_place,top", [(True, 3000), (False, 3000), (True, 33_000)])
+@pytest.mark.parametrize("older,pick,most", [
+    (2501, 1, [float("inf")] * 2), (2502, 1, [3e38, float("inf"), float("inf"), 2.5e38]),
+    (2503, 3, [2e38 + 1e36 * i for i in range(9)]), (2501, 2400, [float("inf")] * 9)])
+def test_eviction_of_negative_beside_infinite_weights(gla_ctx, t, in_place, top, older, pick, most):
+    """Weights from below zero to the largest: the keys' range is all but all of 32 bits, and
+    the filling keys behind an odd number of weights are not in it."""
+    g, n_kv, hd, recent = rng(33, older, top), 2, 64, 5
+    lens = [older + recent, older + recent]
+    w = []
+    for low in (-5.0, -0.3):
+        x = normal(g, n_kv, top).clamp(-0.2, 4.0)
+        x[:, 3] = low
+        x[:, 100:100 + 20 * len(most):20] = torch.tensor(most, device="cuda")
+        w.append(x)
+    evict_and_check(gla_ctx, g, t, in_place, n_kv, hd, lens, w, pick + recent, recent, top)
