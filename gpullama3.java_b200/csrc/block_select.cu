@@ -21,8 +21,10 @@
 //     that was not), those below vmin - 2E surely not, and the few between are
 //     summed again in FP64 (an FP32 query times an FP16 or FP32 bound is exact
 //     there up to 2^-53) and ranked by that.
-// M = 0 (a zero query, zero bounds) means that the FP32 scores are exact; a
-// bound or query too large for E to be finite leaves everything to step 3.
+// M = 0 (a zero query, zero bounds, no channel with both) means that the FP32 scores
+// are exact; where a product of M falls below FP32's normal range its smallest normal
+// number stands for it, and 2E has room for what the scores' own products lose there.
+// A bound or query too large for E to be finite leaves everything to step 3.
 //
 // A cluster of S CTAs works on one (sequence, kv head): each scores a
 // contiguous range of blocks and stores the keys into rank 0's shared memory,
@@ -36,6 +38,7 @@
 // blocks, 8 kv heads, FP32 21 us (FP64 scores throughout: 40; copies of 16 bytes a
 // lane instead of bulk ones: 24).
 #include <algorithm>
+#include <cfloat>
 
 #include "cache_ops.cuh"
 
@@ -322,7 +325,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       upk2(co[e][h / 2], a, b2);
       cs += fabsf(h % 2 ? b2 : a);
     }
-    cs = cs == 0.f ? 0.f : cs * big;  // an infinite bound that no coefficient meets
+    const bool none = cs == 0.f;  // an infinite bound that no coefficient meets
+    cs = none ? 0.f : cs * big;
+    if (!none && big != 0.f) cs = cs < FLT_MIN ? FLT_MIN : cs;  // 0 only if all products are
 #pragma unroll
     for (int m = kLanes / 2; m > 0; m >>= 1) cs += __shfl_xor_sync(0xffffffffu, cs, m);
     nan_q |= cs != cs;

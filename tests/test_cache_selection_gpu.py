@@ -1,9 +1,12 @@
 """Selections of the long-cache operators where they are counted over several CTAs and at the
 ends of the keys' range, against plain 64-bit restatements: every id and every moved byte."""
+import math
+
+import numpy as np
 import pytest
 import torch
 
-from test_cache_ops_gpu import DT, TYPES, caches, i32, kept64, normal, ok, ptrs, rng
+from test_cache_ops_gpu import DT, TYPES, caches, i32, kept64, normal, ok, ptrs, rng, select64
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +95,38 @@ def test_eviction_of_negative_beside_infinite_weights(gla_ctx, t, in_place, top,
         x[:, 100:100 + 20 * len(most):20] = torch.tensor(most, device="cuda")
         w.append(x)
     evict_and_check(gla_ctx, g, t, in_place, n_kv, hd, lens, w, pick + recent, recent, top)
+
+
+@pytest.mark.parametrize("scale_q,scale_b", [(1e-25, 1e-24), (1e-30, 1e-30), (1e-38, 1e-5), (1e-40, 1.0), (1.0, 1e-42)])
+def test_select_orders_products_below_the_smallest_fp32_number(gla_ctx, scale_q, scale_b):
+    """FP32 products that are all zero or nearly so: the order is still that of the 64-bit sums."""
+    g, nh, n_kv, hd, br, nb = rng(34, int(-100 * math.log10(scale_q * scale_b))), 4, 2, 64, 16, 300
+    bo = (normal(g, nb, n_kv, 2, hd).sort(dim=2)[0].double() * scale_b).float().contiguous()
+    q = (normal(g, 1, nh, hd).double() * scale_q).float()
+    for n_sel in (9, 200):
+        ids = torch.empty(1, n_kv, n_sel, dtype=torch.int32, device="cuda")
+        gla_ctx.block_select(q, ptrs([bo]), i32([nb * br]), nb * br, ids, 1, nh, n_kv, hd, br, n_sel, n_last=0)
+        ok(gla_ctx)
+        want, gap = select64(q[0], bo, nb * br, br, n_sel, 0, 0)
+        # the inputs decide: 128 sums of 2^-53 at a magnitude below 2^9 times the scales
+        assert gap > 1e-11 * scale_q * scale_b
+        np.testing.assert_array_equal(ids[0].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("zero", ["q", "bounds", "apart"])
+def test_select_of_exact_zeros_takes_the_lowest_blocks(gla_ctx, zero):
+    """A zero query, zero bounds, and queries and bounds that meet in no channel."""
+    g, nh, n_kv, hd, br, nb, n_sel = rng(35), 4, 2, 128, 16, 300, 20
+    bo = normal(g, nb, n_kv, 2, hd).sort(dim=2)[0].contiguous()
+    q = normal(g, 1, nh, hd)
+    if zero == "q":
+        q[:] = 0.0
+    elif zero == "bounds":
+        bo[:] = 0.0
+    else:
+        q[:, :, ::2] = 0.0
+        bo[:, :, :, 1::2] = 0.0
+    ids = torch.empty(1, n_kv, n_sel, dtype=torch.int32, device="cuda")
+    gla_ctx.block_select(q, ptrs([bo]), i32([nb * br]), nb * br, ids, 1, nh, n_kv, hd, br, n_sel, n_last=0)
+    ok(gla_ctx)
+    assert bool((ids[0].cpu() == torch.arange(n_sel)).all())
