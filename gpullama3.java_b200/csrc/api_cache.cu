@@ -213,10 +213,17 @@ int ensure_scores(gla_ctx* ctx, size_t floats) {
     return fail(ctx, GLA_ERR_INVALID_ARG,
                 "attention workspace must grow; run the largest call once before capture");
   ctx->retired.reserve(ctx->retired.size() + 1);
-  // doubling bounds what outgrown buffers hold to the size of the current one
-  const size_t cap = std::max(floats, 2 * ctx->scores_cap);
+  // doubling bounds what outgrown buffers hold to the size of the current one; where
+  // there is no room for that, what the call needs will do
+  size_t cap = std::max(floats, 2 * ctx->scores_cap);
   void* p = nullptr;
-  if (cudaMalloc(&p, cap * sizeof(float)) != cudaSuccess) {
+  cudaError_t e = cudaMalloc(&p, cap * sizeof(float));
+  if (e != cudaSuccess && cap > floats) {
+    cudaGetLastError();
+    cap = floats;
+    e = cudaMalloc(&p, cap * sizeof(float));
+  }
+  if (e != cudaSuccess) {
     cudaGetLastError();
     return fail(ctx, GLA_ERR_OUT_OF_MEMORY, "attention workspace allocation failed");
   }

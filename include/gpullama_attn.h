@@ -596,8 +596,11 @@ int32_t gla_decode_blocks_f16kv(gla_ctx* ctx, const float* q, const uint16_t* co
  * w = weight_ptrs[b], FP32 [n_kv_heads][weight_stride], weight_stride >= max_n_pos.
  * Entries at and past n_pos are left as they were; set a row's entry to 0 when the
  * row is appended.  Batch entries must not share weights.  Uses a context workspace
- * of batch * n_heads * max_n_pos floats, and up to half as much again for the parts
- * of long sequences, grown on first use (not during stream capture). */
+ * of at most batch * n_heads * (1.51 * max_n_pos + 145) floats (the scores and the parts
+ * of long sequences), grown on first use (not during stream capture): to twice its last
+ * size where that fits, else to what the call needs.  Captured graphs may name outgrown
+ * workspaces, which live until gla_destroy; with them a context that grows by doubling
+ * holds less than four times its largest call's. */
 int32_t gla_decode_weights_f32kv(gla_ctx* ctx, const float* q, const float* const* k_ptrs,
                                  const float* const* v_ptrs, const int32_t* n_pos,
                                  int32_t max_n_pos, float* xb, float* const* weight_ptrs,

@@ -138,3 +138,45 @@ def test_append_of_several_rows_of_one_cache(gla_ctx, t, style):
         assert torch.equal(bo[r // br, :, 0], lo) and torch.equal(bo[r // br, :, 1], hi)
         old[r // br] = bo[r // br]
     assert torch.equal(bo, old)  # the other blocks: as they were
+
+
+def test_the_workspace_grows_in_a_nearly_full_device():
+    """Where twice the last size does not fit, the call's own size does; where that does not fit
+    either, the call is refused and the context goes on."""
+    g, nh, n_kv, hd, n = rng(45), 8, 1, 64, 100
+    k, v = caches(g, [n], n_kv, hd, "f16"), caches(g, [n], n_kv, hd, "f16")
+    kp, vp, np_ = ptrs(k), ptrs(v), i32([n])
+    q, xb = normal(g, 1, nh, hd), torch.empty(1, nh, hd, device="cuda")
+    w = torch.zeros(n_kv, n, device="cuda")
+    wp = ptrs([w])
+    rows = 1 << 25  # times 8 heads in FP32: 1 GiB of scores
+    want, p = attend64(q[0], k[0][:n, :hd], v[0][:n, :hd], hd ** -0.5)
+    tol, rel = attention_bound(q[0], k[0][:n, :hd], v[0][:n, :hd], hd ** -0.5)
+    ctx = gla.Context(0, torch.cuda.current_stream().cuda_stream)
+
+    def call(top):
+        xb.fill_(float("nan"))
+        w.zero_()
+        ctx.decode_weights(q, kp, vp, np_, top, xb, wp, top, 1, nh, n_kv, hd, f16_cache=True)
+        assert ctx.device_status() == 0
+        assert float((xb[0].double() - want).abs().max()) <= tol
+        assert bool(((w[0].double() - p).abs() <= rel * p + 2 * 2.0 ** -24 * p + 1e-37).all())
+
+    try:
+        torch.cuda.empty_cache()
+        free = torch.cuda.mem_get_info()[0]
+        if free < 4 << 30:
+            pytest.skip("not enough device memory")
+        fill = torch.empty(free - (11 << 28), dtype=torch.uint8, device="cuda")  # 2.75 GiB are left
+        call(rows)
+        assert 5 << 28 < torch.cuda.mem_get_info()[0] < 2 << 30  # twice the size does not fit
+        call(rows + (1 << 20))
+        with pytest.raises(gla.GlaError) as e:
+            call(4 * rows)
+        assert e.value.status == -8
+        call(rows + (1 << 20))
+        call(n)
+    finally:
+        fill = None
+        ctx.close()
+        torch.cuda.empty_cache()
