@@ -488,7 +488,8 @@ class Context:
     def decode_blocks(self, q, k_ptrs, v_ptrs, n_pos, block_ids, n_sel, xb, batch, n_heads,
                       n_kv_heads, head_dim, block_rows, scale=None, kv_stride=None,
                       f16_cache=False):
-        """gla_decode_blocks_*: attention over the listed blocks of rows."""
+        """gla_decode_blocks_*: attention over the listed blocks of rows (n_pos must not exceed
+        the caches: there is no max_n_pos to clamp it to)."""
         if scale is None:
             scale = 1.0 / math.sqrt(head_dim)
         if kv_stride is None:

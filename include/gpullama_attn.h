@@ -9,8 +9,8 @@
  *  - Return value: GLA_OK (0) or a negative GLA_ERR_* code.  Nothing aborts and
  *    no C++ exception crosses the ABI.  gla_last_error() describes the last
  *    failure of a context.  Errors found by a kernel while it runs (a bounded
- *    wait that gave up) are latched in a device status word that
- *    gla_device_status() reads back.
+ *    wait that gave up, a bad length or pointer in device memory) are latched
+ *    in a device status word that gla_device_status() reads back.
  *  - A context is not thread-safe: use one per (device, host thread).
  *  - All element offsets are 64-bit.
  *  - Layouts follow the reference:
@@ -84,8 +84,9 @@ int32_t gla_set_stream(gla_ctx* ctx, void* cuda_stream);
 const char* gla_last_error(const gla_ctx* ctx);
 
 /* Synchronises the context's stream, then returns (and clears) the device
- * status word that kernels set when a bounded wait gives up
- * (GLA_OK or GLA_ERR_TIMEOUT), or GLA_ERR_CUDA if the stream itself failed. */
+ * status word that kernels set when a bounded wait gives up (GLA_ERR_TIMEOUT) or a
+ * length or pointer in device memory is bad (GLA_ERR_INVALID_ARG, GLA_ERR_ALIGNMENT);
+ * GLA_OK if none did, GLA_ERR_CUDA if the stream itself failed. */
 int32_t gla_device_status(gla_ctx* ctx, int32_t* device_status);
 
 /* Grows the context workspace so that later decode calls of up to
@@ -499,15 +500,25 @@ int32_t gla_rope_append_f32(gla_ctx* ctx, float* q, float* k, const float* v, fl
  *    128; kvMul = n_heads / n_kv_heads at most 8; any batch.
  *  - n_pos: DEVICE int32 [batch], the rows a sequence has, 0 to max_n_pos (host).
  *    A value outside is clamped and latches GLA_ERR_INVALID_ARG in the device
- *    status.  Rows at and past n_pos are never read nor written, so what they
- *    hold (an infinity, a NaN) does not matter.  Attended rows must be finite.
+ *    status.  gla_decode_blocks_* takes no max_n_pos: a negative length is clamped
+ *    and latched, a length past the cache's end is not seen and its rows are read,
+ *    so the caller passes none (after an append that a full cache refused, too).
+ *    Rows at and past n_pos are never read nor written, so what they hold (an
+ *    infinity, a NaN) does not matter.
+ *  - Attended rows must be finite; of FP32 caches, and their queries, every value, the
+ *    sum of a row's |q k| and the sum of |v| over the rows must lie below 2^127.
+ *  - Attention products have FP32 sums.  FP16 caches: their values are exact, q and
+ *    the softmax weights enter as two FP16 halves (22 bits; weights below 2^-17 of the
+ *    largest are held to 2^-40 of it).  FP32 caches: q, keys, values and weights enter
+ *    as two TF32 halves, which may drop the last of 24 bits, so a single attended row
+ *    comes out within 2^-23 of its values, not always bit for bit.
  *  - block_rows (16, 32, 64 or 128): block j is rows [j*block_rows, (j+1)*block_rows).
  *  - Results do not depend on timing: two calls on the same input give the
  *    same bits.
  *  - Calls can be captured in a CUDA graph; gla_decode_weights_* and long lists of
  *    gla_decode_blocks_* use a context workspace that must have grown before (run
  *    the largest call once), so graphs of one context that hold them must not run at
- *    the same time. */
+ *    the same time; nor must such calls before and after a gla_set_stream. */
 
 /* bounds: [n_blocks][n_kv_heads][2][head_dim] a sequence: the smallest (0) and the
  * largest (1) key of each channel over the rows t < n_pos of a block.  Exact; a NaN
