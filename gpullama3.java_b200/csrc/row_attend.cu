@@ -1060,7 +1060,9 @@ size_t attend_workspace_floats(const AttendRequest& r, const DeviceInfo& dev) {
                            : part_rows_for(r.batch, r.n_kv, rows, unit, dev);
   const int64_t parts = part ? (rows + part - 1) / part : 0;
   const int64_t pitch = r.block_ids ? 0 : score_pitch_for(rows);
-  return (size_t)r.batch * r.n_heads * (size_t)(pitch + parts * (r.head_dim + 2));
+  const size_t heads = (size_t)r.batch * r.n_heads, each = (size_t)(pitch + parts * (r.head_dim + 2));
+  constexpr size_t kMost = SIZE_MAX / 8;  // no device holds it: the allocation fails
+  return each && heads > kMost / each ? kMost : heads * each;
 }
 
 int launch_attend(const AttendRequest& r, const DeviceInfo& dev, cudaStream_t stream,

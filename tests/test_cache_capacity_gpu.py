@@ -180,3 +180,13 @@ def test_the_workspace_grows_in_a_nearly_full_device():
         fill = None
         ctx.close()
         torch.cuda.empty_cache()
+
+
+def test_a_workspace_past_64_bits_is_refused(gla_ctx):
+    """2^33 heads of 2^31 scores: the count itself would wrap to nothing.  Refused before any launch."""
+    p, n = torch.zeros(4, dtype=torch.int64, device="cuda"), i32([0])
+    x = torch.zeros(512, device="cuda")
+    with pytest.raises(gla.GlaError) as e:
+        gla_ctx.decode_weights(x, p, p, n, (1 << 31) - 1, x, p, (1 << 31) - 1, 1 << 30, 8, 1, 64)
+    assert e.value.status == -8
+    ok(gla_ctx)
