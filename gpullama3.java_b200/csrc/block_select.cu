@@ -166,13 +166,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   __shared__ uint64_t s_near_key[kNear];
   __shared__ int32_t s_near_n, s_sure_n;
   __shared__ uint64_t s_bar[kWarps * Sh::kStages];
-  __shared__ int s_abort;  // a bounded wait gave up
+  __shared__ int s_abort, s_late;  // a bounded wait gave up; so did one for what it left
+  __shared__ int32_t s_lost[kWarps];  // of a warp whose wait gave up: that step
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = S > 1 ? (int)(blockIdx.x % (unsigned)S) : 0;
   const int item = (int)(blockIdx.x / (unsigned)S);
   const int b = item / n_kv, g = item - b * n_kv;
   const int G = n_heads / n_kv;
-  if (tid == 0) s_abort = 0;
+  if (tid == 0) s_abort = s_late = 0;
   pdl_wait();
   pdl_launch_dependents();
   // q, the length and the pointer are loaded side by side
@@ -254,12 +255,15 @@ __global__ void __launch_bounds__(kThreads, 2)
   bool strange = false;  // a NaN bound (its scores are NaN; a maximum would drop it)
   uint32_t kmin = ~0u, kmax = 0;
   uint32_t phase = 0;  // parity of the ring's round
+  // A wait that gave up (the status word says so) ends the warp's copies: what it scores
+  // from then on is arbitrary, but every block gets a key.
+  bool alive = true;
   for (int32_t jw0 = w0; jw0 < hi; jw0 += kStages * kStep, phase ^= 1) {
 #pragma unroll
     for (int st = 0; st < kStages; ++st) {
       const int32_t jw = jw0 + st * kStep, j0 = jw + sub * kBlk;
       if (jw >= hi) break;
-      mbar_wait(bars + st, phase, &s_abort, status);
+      const bool here = mbar_wait(bars + st, phase, &s_abort, status);
       float acc[kVals];
 #pragma unroll
       for (int i = 0; i < kBlk; ++i) {
@@ -290,8 +294,13 @@ __global__ void __launch_bounds__(kThreads, 2)
           if (GP > 1) acc[i * GP + (2 * h + 1) % GP] = b2;
         }
       }
-      __syncwarp();  // read out by every lane
-      fetch(st, jw + kStages * kStep);
+      if (alive) {
+        alive = __all_sync(0xffffffffu, here);  // and read out by every lane
+        if (alive)
+          fetch(st, jw + kStages * kStep);
+        else
+          s_lost[warp] = (jw - w0) / kStep;
+      }
       const float s = reduce_scatter<kVals, kLanes>(acc, sl);
       // lane sl holds value sl >> kRep: block value / GP, head value % GP
       constexpr int kRep = ilog2(kLanes) - ilog2(kVals);
@@ -309,6 +318,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (h == 0 && (sl & ((1 << kRep) - 1)) == 0) key0[j] = key;
       }
     }
+  }
+  if (!alive) {  // no copy may land after the CTA has left
+    __syncwarp();
+    for (int32_t i = s_lost[warp], e = i + kStages; i < e && w0 + i * kStep < hi; ++i)
+      mbar_wait(bars + i % kStages, (i / kStages) & 1, &s_late, status);
   }
   // M of this warp's blocks (its lane groups see different blocks: their maximum counts)
   if (strange) big = INFINITY;
