@@ -10,8 +10,8 @@
 // Latency-bound: a token is a few tens of KB.  What costs is the chain of
 // double pow, cos and sin; the (cos, sin) pairs of a position are computed
 // once per CTA, one pair a thread, and shared by its heads, and the CTAs of
-// one sequence take kHeadsPerCta heads each.  Measured on one B200: 3.1 us for one
-// sequence of the 1B shape, 5.2 us for 96 of the 8B shape, with bounds.
+// one sequence take kHeadsPerCta heads each.  Measured on one B200: 3.3 to 3.8 us
+// for one sequence of the 1B shape, 5.2 us for 96 of the 8B shape, with bounds.
 #include "cache_ops.cuh"
 #include "gla_rope.cuh"
 

@@ -33,9 +33,9 @@
 // One launch, no global workspace.
 //
 // HBM-bound for a batch, latency-bound for a token.  Measured on one B200: 2048
-// blocks of 4 kv heads, FP16, 11.0 us, of which 3 until the first bounds are here, 3
+// blocks of 4 kv heads, FP16, 11.1 us, of which 3 until the first bounds are here, 3
 // scoring, 1 the cluster's barrier and 4 the selection; 16 sequences of up to 1024
-// blocks, 8 kv heads, FP32 21 us (FP64 scores throughout: 40; copies of 16 bytes a
+// blocks, 8 kv heads, FP32 21.5 us (FP64 scores throughout: 40; copies of 16 bytes a
 // lane instead of bulk ones: 24).
 #include <algorithm>
 #include <cfloat>

@@ -16,9 +16,9 @@
 // Calls of few kv heads do both in one launch (evict_small_kernel).
 //
 // Measured on one B200: 4096 rows of 8 kv heads to 1024, FP32, 8.4 us (a chain of loads
-// and passes); 16 sequences of up to 32,768 FP16 rows to 4096 110 us, 21
+// and passes); 16 sequences of up to 32,768 FP16 rows to 4096 111 us, 21
 // the selection (the longest sequence's walks) and 87 the copy (6.2 TB/s read and
-// written); the same in place 151 us (16 of exactly 32,768 rows; one CTA a head and
+// written); the same in place 149 us (16 of exactly 32,768 rows; one CTA a head and
 // 64 columns of K or V: 209).
 #include <algorithm>
 

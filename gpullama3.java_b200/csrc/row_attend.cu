@@ -44,8 +44,8 @@
 // Measured on one B200: listed blocks, 64 of 64 FP16 rows for 4 kv heads of 128
 // 8.6 us (latency: 131 KB an SM through 64 bytes a clock, then the joins); 256
 // queries over one cache of 32,768 rows, 32 blocks each, 220 us (2.1 GB through L2,
-// 9.8 TB/s); 64 separate FP16 caches 105 us, 5.1 TB/s.  Weights, 131,072 FP16 rows of
-// 4 kv heads 60 us (4.6 TB/s with scores and weights).
+// 9.8 TB/s, as every query and kv head reads its own rows); 64 separate FP16 caches 105 us, 5.1 TB/s.  Weights, 131,072 FP16 rows of
+// 4 kv heads 58 us (4.7 TB/s with scores and weights).
 #include <cmath>
 
 #include "cache_ops.cuh"

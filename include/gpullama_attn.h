@@ -505,8 +505,9 @@ int32_t gla_rope_append_f32(gla_ctx* ctx, float* q, float* k, const float* v, fl
  *    so the caller passes none (after an append that a full cache refused, too).
  *    Rows at and past n_pos are never read nor written, so what they hold (an
  *    infinity, a NaN) does not matter.
- *  - Attended rows must be finite; of FP32 caches, and their queries, every value, the
- *    sum of a row's |q k| and the sum of |v| over the rows must lie below 2^127.
+ *  - Attended rows and queries must be finite and |scale q| below 2^126; of FP32 caches
+ *    and their queries every value, the sum of a row's |q k| and the sum of |v| over the
+ *    rows must lie below 2^127.
  *  - Attention products have FP32 sums.  FP16 caches: their values are exact, q and
  *    the softmax weights enter as two FP16 halves (22 bits; weights below 2^-17 of the
  *    largest are held to 2^-40 of it).  FP32 caches: q, keys, values and weights enter
